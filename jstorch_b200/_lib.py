@@ -15,6 +15,9 @@ LIB_PATH = PKG / "libjstorch_gemm.so"
 HEADER = PKG.parent / "include" / "jstorch_gemm.h"
 CONV_HEADER = PKG.parent / "include" / "jstorch_conv.h"
 RNN_HEADER = PKG.parent / "include" / "jstorch_rnn.h"
+SCAN_HEADER = PKG.parent / "include" / "jstorch_scan.h"
+DROPOUT_HEADER = PKG.parent / "include" / "jstorch_dropout.h"
+QUANT_HEADER = PKG.parent / "include" / "jstorch_quant.h"
 
 JST_OK = 0
 STATUS_NAMES = {
@@ -49,6 +52,19 @@ class GemmDesc(ctypes.Structure):
         ("kernel", ctypes.c_int),
         ("stream", ctypes.c_void_p),
         ("aux", ctypes.c_void_p), ("ld_aux", ctypes.c_int64), ("stride_aux", ctypes.c_int64),
+    ]
+
+
+class GemmI8Desc(ctypes.Structure):
+    """Mirror of `jst_gemm_i8_desc` (field order and C types must match)."""
+    _fields_ = [
+        ("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int),
+        ("A", ctypes.c_void_p), ("lda", ctypes.c_int64),
+        ("B", ctypes.c_void_p), ("ldb", ctypes.c_int64),
+        ("a_scale", ctypes.c_void_p), ("b_scale", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("epilogue", ctypes.c_int),
+        ("C", ctypes.c_void_p), ("ldc", ctypes.c_int64),
+        ("stream", ctypes.c_void_p),
     ]
 
 
@@ -127,6 +143,19 @@ def load() -> ctypes.CDLL:
     lib.jst_gru_layer_backward.restype = ci
     lib.jst_gru_layer_backward.argtypes = ([vp, ci, ci, ci, ci, vp, vp, vp, ci, vp, ctypes.c_int64, vp, vp,
                                             ctypes.c_int64, vp] + [vp] * 6 + [ci, vp])
+    i64, u64 = ctypes.c_int64, ctypes.c_uint64
+    lib.jst_scan_forward.restype = ci
+    lib.jst_scan_forward.argtypes = [vp, i64, ci, ci, ci, vp, vp, ci, ci, vp, i64, vp, vp]
+    lib.jst_scan_backward.restype = ci
+    lib.jst_scan_backward.argtypes = [vp, i64, ci, ci, ci, vp, vp, ci, ci, vp, i64, vp, i64, vp, vp, i64, vp, vp]
+    lib.jst_dropout.restype = ci
+    lib.jst_dropout.argtypes = [vp, i64, vp, i64, i64, i64, ctypes.c_double, u64, u64, vp, vp]
+    lib.jst_quantize_rows_i8.restype = ci
+    lib.jst_quantize_rows_i8.argtypes = [vp, i64, ci, ci, vp, i64, vp, vp]
+    lib.jst_gemm_i8.restype = ci
+    lib.jst_gemm_i8.argtypes = [ctypes.POINTER(GemmI8Desc)]
+    lib.jst_linear_i8.restype = ci
+    lib.jst_linear_i8.argtypes = [vp, i64, ci, ci, vp, i64, vp, ci, vp, ci, vp, i64, vp]
     _lib = lib
     return lib
 
@@ -163,6 +192,67 @@ def check(status: int) -> None:
 def check_last() -> None:
     """Raise if the last void launcher on this thread failed."""
     check(load().jst_get_last_status())
+
+
+def require_f32(x, name: str) -> None:
+    """Raise unless x is a float32 CUDA tensor."""
+    import torch
+
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32 (got {x.dtype})")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device")
+
+
+def stream_of(device, stream) -> int:
+    """The handle of `stream`, by default torch's current stream of `device`."""
+    if stream is None:
+        import torch
+
+        return torch.cuda.current_stream(device).cuda_stream
+    if stream.device != device:
+        raise ValueError(f"stream belongs to {stream.device}, the tensors to {device}")
+    return stream.cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on(device):
+    """A context with `device` current; nothing to do where it is already."""
+    import torch
+
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def empty(shape, device, stream, dtype=None):
+    """An uninitialised tensor (float32 by default) that belongs to `stream`:
+    memory that torch's allocator reuses in another stream's order could still
+    be in use there when `stream` writes it."""
+    import torch
+
+    dtype = dtype or torch.float32
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def launch(device, stream, name: str, *args) -> None:
+    """Call the entry point `name` on `stream` with `device` current."""
+    handle = stream_of(device, stream)
+    with on(device):
+        check(getattr(load(), name)(*args, handle))
 
 
 def header_functions(header: Path = HEADER) -> list[str]:

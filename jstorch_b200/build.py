@@ -5,7 +5,7 @@
     python -m jstorch_b200.build --ptxas-v  # print register / spill / smem use
 
 Outputs (git-ignored, shipped with the source tree):
-    jstorch_b200/libjstorch_gemm.so   the C-ABI GEMM library (include/jstorch_gemm.h, jstorch_conv.h)
+    jstorch_b200/libjstorch_gemm.so   the C-ABI GEMM library (include/jstorch_{gemm,conv,rnn,scan,dropout,quant}.h)
     jstorch_b200/_core*.so            the host core (Tensor / GradTensor), Python extension
     jstorch_b200/libjstorch_dist.so   the NCCL sharded GEMMs (include/jstorch_dist.h)
 
@@ -34,7 +34,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
            "--expt-relaxed-constexpr", "-DNDEBUG", f"-I{INCLUDE}"] + ARCH
 
-GEMM_SOURCES = ["gemm_api.cu", "gemm_ffma.cu", "gemm_tc.cu", "splitk.cu", "conv.cu", "gru.cu", "hostio.cu", "profile.cu"]
+GEMM_SOURCES = ["gemm_api.cu", "gemm_ffma.cu", "gemm_tc.cu", "splitk.cu", "conv.cu", "gru.cu", "hostio.cu", "profile.cu",
+                "dropout.cu", "scan.cu", "quant.cu"]
 GEMM_HEADERS = ["gemm_internal.h", "ptx.cuh"]
 GEMM_LIB = PKG / "libjstorch_gemm.so"
 
@@ -60,7 +61,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 def build_gemm(force: bool = False, ptxas_v: bool = False, verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
-    headers = [CSRC / h for h in GEMM_HEADERS] + [INCLUDE / "jstorch_gemm.h", INCLUDE / "jstorch_conv.h", INCLUDE / "jstorch_rnn.h"]
+    headers = [CSRC / h for h in GEMM_HEADERS] + [INCLUDE / f"jstorch_{n}.h" for n in
+                                                  ("gemm", "conv", "rnn", "scan", "dropout", "quant")]
     objs = []
     for src in GEMM_SOURCES:
         s = CSRC / src
@@ -90,7 +92,7 @@ def build_core(force: bool = False, verbose: bool = False) -> Path:
     import pybind11
 
     BUILD.mkdir(exist_ok=True)
-    headers = [CORE / h for h in CORE_HEADERS] + [INCLUDE / "jstorch_gemm.h"]
+    headers = [CORE / h for h in CORE_HEADERS] + [INCLUDE / "jstorch_gemm.h", INCLUDE / "jstorch_dropout.h"]
     objs = []
     incs = [f"-I{INCLUDE}", f"-I{CUDA_HOME}/include", f"-I{sysconfig.get_paths()['include']}",
             f"-I{pybind11.get_include()}"]

@@ -110,6 +110,18 @@ GradPtr GradTensor::relu_() {
         {shared_from_this()});
 }
 
+// d/dx of x * keep / (1 - p) is the same function of the upstream gradient.
+GradPtr GradTensor::dropout_(double p, uint64_t seed, uint64_t offset) {
+    Tensor out = data.dropout(p, seed, offset);
+    if (!requires_grad) return make(std::move(out));
+    return make_with_grad(
+        std::move(out),
+        [p, seed, offset](const Tensor& g, const std::vector<bool>&) {
+            return std::vector<Tensor>{g.dropout(p, seed, offset)};
+        },
+        {shared_from_this()});
+}
+
 GradPtr GradTensor::transpose_() {
     Tensor out = data.transpose();
     if (!requires_grad) return make(std::move(out));

@@ -47,6 +47,7 @@ class GradTensor : public std::enable_shared_from_this<GradTensor> {
     GradPtr matmul_(const GradPtr& other);   // autograd.hpp:433-441
     GradPtr add_(const GradPtr& other);      // autograd.hpp:334-342 (+ unbroadcast :324-332)
     GradPtr relu_();                         // autograd.hpp:127-134
+    GradPtr dropout_(double p, uint64_t seed, uint64_t offset);  // the gradient draws the same mask again
     GradPtr transpose_();                    // autograd.hpp:532-538
     GradPtr transpose_(int d0, int d1);      // autograd.hpp:524-530
 

@@ -81,6 +81,7 @@ PYBIND11_MODULE(_core, m) {
             }, py::arg("weight"), py::arg("bias") = py::none())
         .def("add", &Tensor::add)
         .def("relu", &Tensor::relu)
+        .def("dropout", &Tensor::dropout, py::arg("p"), py::arg("seed"), py::arg("offset") = 0)
         .def("sum", &Tensor::sum, py::arg("dim"), py::arg("keepdim") = false)
         .def("transpose", [](const Tensor& t, py::args dims) {
                 if (dims.size() == 0) return t.transpose();
@@ -107,6 +108,9 @@ PYBIND11_MODULE(_core, m) {
         .def("matmul", [](GradTensor& self, const py::object& o) { return self.shared_from_this()->matmul_(as_grad(o)); })
         .def("add", [](GradTensor& self, const py::object& o) { return self.shared_from_this()->add_(as_grad(o)); })
         .def("relu", [](GradTensor& self) { return self.shared_from_this()->relu_(); })
+        .def("dropout", [](GradTensor& self, double p, uint64_t seed, uint64_t offset) {
+                return self.shared_from_this()->dropout_(p, seed, offset);
+            }, py::arg("p"), py::arg("seed"), py::arg("offset") = 0)
         .def("transpose", [](GradTensor& self, py::args dims) {
                 if (dims.size() == 0) return self.shared_from_this()->transpose_();
                 if (dims.size() == 2) return self.shared_from_this()->transpose_(dims[0].cast<int>(), dims[1].cast<int>());

@@ -7,6 +7,7 @@
 #include <sstream>
 #include <stdexcept>
 
+#include "../../../include/jstorch_dropout.h"
 #include "../../../include/jstorch_gemm.h"
 #include "core_kernels.h"
 
@@ -340,6 +341,15 @@ Tensor Tensor::relu_backward(const Tensor& x) const {
     Tensor r(shape_);
     core::relu_backward(g.data(), xc.data(), r.data(), size(), g_stream);
     check_cuda(cudaPeekAtLastError(), "relu_backward");
+    return r;
+}
+
+Tensor Tensor::dropout(double p, uint64_t seed, uint64_t offset) const {
+    const Tensor a = contiguous();
+    Tensor r(shape_);
+    const int64_t n = size();
+    check_jst(jst_dropout(a.data(), n, r.data(), n, 1, n, p, seed, offset, nullptr,
+                          reinterpret_cast<jst_stream_t>(g_stream)), "dropout");
     return r;
 }
 

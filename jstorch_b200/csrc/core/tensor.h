@@ -69,6 +69,8 @@ class Tensor {
     Tensor add(const Tensor& other) const;  // same shape, or [..., N] + [N] (binary.cu)
     Tensor relu() const;                    // kernels.cuh:50
     Tensor relu_backward(const Tensor& x) const;  // this * (x > 0)  (autograd.hpp:132)
+    // jst_dropout of the elements in row-major order (include/jstorch_dropout.h)
+    Tensor dropout(double p, uint64_t seed, uint64_t offset) const;
     Tensor sum(int dim, bool keepdim) const;      // dim 0 of 2-D; other dims via transpose
 
   private:

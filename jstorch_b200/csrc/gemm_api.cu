@@ -86,6 +86,11 @@ static int current_device(int* out_dev) {
     return JST_OK;
 }
 
+int require_device() {
+    int dev = 0;
+    return current_device(&dev);
+}
+
 uint32_t* device_error_word() {
     int dev = 0;
     cudaGetDevice(&dev);

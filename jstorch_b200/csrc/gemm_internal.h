@@ -54,6 +54,15 @@ inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 bl
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// JST_OK when the current device is one this library runs on (sets it up once).
+int require_device();
+
+// Whether [a, a + na) and [b, b + nb) (bytes) have a byte in common.
+inline bool ranges_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
 // Stream-ordered scratch from the library's per-device pool (checks the device first).
 int workspace_alloc(size_t bytes, cudaStream_t s, void** out);
 int workspace_free(void* p, cudaStream_t s);
@@ -139,6 +148,10 @@ enum KernelId {
     KID_CONV,  // im2col / col2im / permute of the convolution launchers
     KID_SPLITK_REDUCE,
     KID_RNN,  // GRU gate kernel
+    KID_SCAN,
+    KID_DROPOUT,
+    KID_QUANT,    // row quantisation, realignment of 8-bit rows
+    KID_GEMM_I8,
     KERNEL_ID_COUNT
 };
 

@@ -34,7 +34,8 @@ std::vector<cudaEvent_t> g_free_events;
 Stat g_stats[KERNEL_ID_COUNT];
 
 const char* kKernelNames[KERNEL_ID_COUNT] = {"tc_gemm", "split_rows", "split_transpose", "ffma_gemm",
-                                             "fill_epilogue", "conv_im2col", "splitk_reduce", "gru_gate"};
+                                             "fill_epilogue", "conv_im2col", "splitk_reduce", "gru_gate",
+                                             "scan", "dropout", "quantize_rows", "gemm_i8"};
 
 cudaEvent_t take_event() {
     if (!g_free_events.empty()) {

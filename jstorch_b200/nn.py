@@ -40,6 +40,16 @@ class Module:
             m._init_grad()
         return self
 
+    def train(self, mode: bool = True) -> "Module":
+        """Set `training` here and in every submodule (Dropout acts on it)."""
+        self.training = mode
+        for m in self._modules.values():
+            m.train(mode)
+        return self
+
+    def eval(self) -> "Module":
+        return self.train(False)
+
     def load_state_dict(self, state: dict, prefix: str = "") -> None:
         """nn.js:58-80: replace parameters by key (call _init_grad afterwards)."""
         for name in list(self._parameters):
@@ -79,6 +89,27 @@ class ReLU(Module):
 
     def forward(self, x):
         return x.relu()
+
+
+class Dropout(Module):
+    """Drops elements with probability p while training, the identity otherwise.
+
+    The mask of the n-th training call is that of (seed, offset + n)
+    (include/jstorch_dropout.h) and is not stored: give the Dropouts of a model
+    different seeds.  The reference's nn.js has no such module."""
+
+    def __init__(self, p: float = 0.5, seed: int = 0, offset: int = 0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be in [0, 1] (got {p})")
+        self.p, self.seed, self.offset = p, seed, offset
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        y = x.dropout(self.p, self.seed, self.offset)
+        self.offset += 1
+        return y
 
 
 class Sequential(Module):

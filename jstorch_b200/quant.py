@@ -1,0 +1,120 @@
+"""8-bit integer matrix products (include/jstorch_quant.h) on torch CUDA tensors:
+one scale a token, one scale a channel, exact integer sums.
+
+    q, s = quantize_rows(w)                      # a weight [out, in], once
+    y = linear_i8(x, q, s, bias=b)               # fp32 rows in and out
+    y = gemm_i8(xq, q, x_scale, s, bias=b)       # rows quantised before
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import _lib
+
+
+def _int8_rows(x, name: str):
+    """(rows, cols, pitch) of a 2-D int8 CUDA tensor whose columns are adjacent."""
+    import torch
+
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dtype != torch.int8:
+        raise TypeError(f"{name} must be int8 (got {x.dtype})")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device")
+    return _matrix(x, name)
+
+
+def _matrix(x, name: str):
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be 2-D")
+    rows, cols = x.shape
+    pitch, unit = x.stride()
+    if (cols > 1 and unit != 1) or (rows > 1 and pitch < cols):
+        raise ValueError(f"{name}: unsupported strides {tuple(x.stride())} for shape {tuple(x.shape)}")
+    return rows, cols, pitch if rows > 1 else max(cols, 1)
+
+
+def _vector(v, name: str, n: int, device):
+    _lib.require_f32(v, name)
+    if v.shape != (n,) or v.device != device or (n > 1 and v.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous float32 tensor with {n} elements on {device}")
+    return v.data_ptr()
+
+
+def _output(out, M: int, N: int, device, stream):
+    if out is None:
+        return _lib.empty((M, N), device, stream), N
+    _lib.require_f32(out, "out")
+    if out.shape != (M, N) or out.device != device:
+        raise ValueError(f"out must be a float32 tensor of shape {(M, N)} on {device}")
+    return out, _matrix(out, "out")[2]
+
+
+def quantize_rows(x, *, stream=None):
+    """(q, scale) of a 2-D float32 CUDA tensor: scale[r] = max|x[r]| / 127 in
+    fp32, q[r] = x[r] / scale[r] to the nearest integer (ties to even) in int8.
+    A row that holds an infinity or a NaN gets scale NaN.  The rows of q start
+    at multiples of 16 bytes (q is a view when x has other widths), as
+    gemm_i8 reads them in place.
+    """
+    import torch
+
+    _lib.require_f32(x, "x")
+    rows, cols, ldx = _matrix(x, "x")
+    pitch = max((cols + 15) // 16 * 16, 16)
+    held = _lib.empty((rows, pitch), x.device, stream, torch.int8)
+    scale = _lib.empty((rows,), x.device, stream)
+    _lib.launch(x.device, stream, "jst_quantize_rows_i8", x.data_ptr(), ldx, rows, cols, held.data_ptr(), pitch,
+                scale.data_ptr())
+    return held[:, :cols], scale
+
+
+def gemm_i8(a, w, a_scale, w_scale, out=None, *, bias=None, relu: bool = False, stream=None):
+    """out[m, n] = relu?(a_scale[m] * w_scale[n] * sum_k a[m, k] * w[n, k] + bias[n]).
+
+    a: [M, K] int8 rows (tokens), w: [N, K] int8 rows (channels, an nn.Linear
+    weight); K <= 131071.  Rows may have a pitch; 16-byte aligned rows are read
+    in place, others are copied first where the tensor cores compute.  out:
+    float32 [M, N] (a pitch is allowed).  Runs asynchronously on `stream`
+    (default: torch's current stream).
+    """
+    M, K, lda = _int8_rows(a, "a")
+    N, Kw, ldw = _int8_rows(w, "w")
+    if K != Kw:
+        raise ValueError(f"gemm_i8 shape mismatch: a is [{M}, {K}], w is [{N}, {Kw}]")
+    if w.device != a.device:
+        raise ValueError("a and w must live on one device")
+    d = _lib.GemmI8Desc()
+    d.M, d.N, d.K = M, N, K
+    d.A, d.lda, d.B, d.ldb = a.data_ptr(), lda, w.data_ptr(), ldw
+    d.a_scale = _vector(a_scale, "a_scale", M, a.device)
+    d.b_scale = _vector(w_scale, "w_scale", N, a.device)
+    d.bias = _vector(bias, "bias", N, a.device) if bias is not None else None
+    d.epilogue = (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0)
+    out, d.ldc = _output(out, M, N, a.device, stream)
+    d.C = out.data_ptr()
+    d.stream = _lib.stream_of(a.device, stream)
+    with _lib.on(a.device):
+        _lib.check(_lib.load().jst_gemm_i8(ctypes.byref(d)))
+    return out
+
+
+def linear_i8(x, w, w_scale, out=None, *, bias=None, relu: bool = False, stream=None):
+    """gemm_i8 of quantize_rows(x): x [M, K] float32 rows (a pitch is allowed),
+    w [N, K] int8 with w_scale [N] (quantize_rows of the weight), out float32
+    [M, N].  The same result as the two calls, in fewer passes.
+    """
+    _lib.require_f32(x, "x")
+    M, K, ldx = _matrix(x, "x")
+    N, Kw, ldw = _int8_rows(w, "w")
+    if K != Kw:
+        raise ValueError(f"linear_i8 shape mismatch: x is [{M}, {K}], w is [{N}, {Kw}]")
+    if w.device != x.device:
+        raise ValueError("x and w must live on one device")
+    ws = _vector(w_scale, "w_scale", N, x.device)
+    b = _vector(bias, "bias", N, x.device) if bias is not None else None
+    out, ldy = _output(out, M, N, x.device, stream)
+    _lib.launch(x.device, stream, "jst_linear_i8", x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, ws, N, b,
+                (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0), out.data_ptr(), ldy)
+    return out

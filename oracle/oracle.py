@@ -443,3 +443,141 @@ def gru_backward_f64(x, params, hidden, num_layers=1, bidirectional=False, h0=No
             grads[f"bias_hh_l{l}{sfx}"] = gb_hh
         g_out = dinp
     return grads, g_out, dh0
+
+
+# ------------------------------------------------- gated linear recurrence
+def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, dh_n=None, with_grads=False):
+    """The recurrence h_t = z h_{t-1} + (1 - z) n, z = sigmoid(a), n = tanh(c)
+    or c, of gates [seq, batch, 2H] = (a | c), step by step in fp64, with its
+    gradients, and for every result a bound of what fp32 arithmetic may be off.
+
+    Returns {name: (value, bound)} for out, h_n and, with_grads, dgates, dh0.
+
+    The bounds carry first-order rounding errors through the recurrence, u =
+    2^-24.  One exponential of -|a| (2 ulp = 4u) gives big = 1 / (1 + e) (its
+    own sum 1u, division 2 ulp = 4u, and e / (1 + e) of e's error) and small =
+    e * big (e's 4u, big's error, 1u), so the larger of z and 1 - z is off by
+    5u + 4u * small and the smaller by 14u, relative.  tanh is 2 ulp = 4u.
+    Each step then rounds a product and a sum, and a scan that composes steps
+    (products of z) rounds once more a step: 3u.  The few compositions of a
+    scan's tree add 16u once.  Below 2^-126 fp32 is a grid of 2^-149: an
+    exponential there is off by 2 of its steps whatever its size and every
+    rounding by half of one, which the factors that they meet carry on: 8
+    steps, 2^-146, a recurrence step times those factors.  m and g are the magnitudes (the same sums of
+    absolute values) that these relative errors apply to.
+    """
+    u, tiny = 2.0 ** -24, 2.0 ** -146
+    gates = np.asarray(gates, dtype=np.float64)
+    seq, batch, hidden = gates.shape[0], gates.shape[1], gates.shape[2] // 2
+    length = np.full(batch, seq) if lengths is None else np.clip(np.asarray(lengths), 0, seq)
+    inside = np.arange(seq)[:, None] < length[None, :]
+    a = np.where(inside[..., None], gates[..., :hidden], 0.0)
+    c = np.where(inside[..., None], gates[..., hidden:], 0.0)
+    e = np.exp(-np.abs(a))
+    big, small = 1 / (1 + e), e / (1 + e)
+    z, rest = np.where(a >= 0, big, small), np.where(a >= 0, small, big)
+    n = np.tanh(c) if tanh else c
+    of_big = 5 + 4 * small
+    cz, cr = np.where(a >= 0, of_big, 14.0), np.where(a >= 0, 14.0, of_big)
+    cn = 4.0 if tanh else 0.0
+    times = range(seq - 1, -1, -1) if reverse else range(seq)
+    h = np.zeros((batch, hidden)) if h0 is None else np.asarray(h0, dtype=np.float64)
+    m, err = np.abs(h), np.zeros((batch, hidden))
+    before, before_m, before_e = np.empty_like(z), np.empty_like(z), np.empty_like(z)
+    out, out_e = np.zeros_like(z), np.zeros_like(z)
+    for t in times:
+        k = inside[t][:, None]
+        before[t], before_m[t], before_e[t] = h, m, err
+        err = np.where(k, z[t] * err + u * ((cz[t] + 3) * z[t] * m + (cr[t] + cn + 3) * rest[t] * np.abs(n[t]))
+                       + tiny * (m + np.abs(n[t]) + 1), err)
+        h = np.where(k, z[t] * h + rest[t] * n[t], h)
+        m = np.where(k, z[t] * m + rest[t] * np.abs(n[t]), m)
+        out[t], out_e[t] = np.where(k, h, 0.0), np.where(k, err + 16 * u * m, 0.0)
+    r = {"out": (out, out_e), "h_n": (h, err + 16 * u * m)}
+    if not with_grads:
+        return r
+    dout = np.zeros_like(z) if dout is None else np.asarray(dout, dtype=np.float64)
+    g = np.zeros((batch, hidden)) if dh_n is None else np.asarray(dh_n, dtype=np.float64)
+    gm, ge = np.abs(g), np.zeros((batch, hidden))
+    dgates, dgates_e = np.zeros_like(gates), np.zeros_like(gates)
+    for t in reversed(times):
+        k = inside[t][:, None]
+        d = np.where(k, dout[t], 0.0)
+        G, Gm = g + d, gm + np.abs(d)
+        Ge = ge + 17 * u * Gm
+        diff = before[t] - n[t]
+        diff_e = before_e[t] + 16 * u * before_m[t] + cn * u * np.abs(n[t]) + u * np.abs(diff)
+        slope = z[t] * rest[t]
+        dn = rest[t] * ((1 - n[t] ** 2) if tanh else 1.0)
+        dgates[t] = np.where(k, np.concatenate([G * diff * slope, G * dn], axis=1), 0.0)
+        dgates_e[t] = np.where(k, np.concatenate([
+            tiny * (Gm + 1) * (np.abs(diff) + 1) + Ge * np.abs(diff) * slope + Gm * slope * (diff_e + np.abs(diff) * (cz[t] + cr[t] + 3) * u),
+            tiny * (Gm + 1) + Ge * dn + Gm * (dn * (cr[t] + 3) * u + (rest[t] * 10 * u if tanh else 0.0))], axis=1), 0.0)
+        ge = np.where(k, z[t] * ge + u * (cz[t] + 4) * z[t] * Gm + tiny * (Gm + 1), ge)
+        g, gm = np.where(k, z[t] * G, g), np.where(k, z[t] * Gm, gm)
+    r["dgates"] = (dgates, dgates_e)
+    r["dh0"] = (g, ge + 16 * u * gm)
+    return r
+
+
+# ------------------------------------------------------------------ dropout
+def philox4x32_10(counter, key):
+    """Words [n, 4] of Philox4x32-10 for counters [n, 4] under a key of two words."""
+    low, shift = np.uint64(0xFFFFFFFF), np.uint64(32)
+    c = [np.asarray(counter, dtype=np.uint64)[:, i] for i in range(4)]
+    k0, k1 = int(key[0]), int(key[1])
+    for _ in range(10):
+        p, q = np.uint64(0xD2511F53) * c[0], np.uint64(0xCD9E8D57) * c[2]
+        c = [(q >> shift) ^ c[1] ^ np.uint64(k0), q & low, (p >> shift) ^ c[3] ^ np.uint64(k1), p & low]
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    return np.stack(c, axis=1).astype(np.uint32)
+
+
+def dropout_keep(n: int, p: float, seed: int, offset: int) -> np.ndarray:
+    """Which of n elements dropout keeps: word i % 4 of counter (i // 4, offset) >= floor(p 2^32)."""
+    if p >= 1.0:
+        return np.zeros(n, dtype=bool)
+    block = np.arange((n + 3) // 4, dtype=np.uint64)
+    full = np.zeros_like(block)
+    counter = np.stack([block & np.uint64(0xFFFFFFFF), block >> np.uint64(32),
+                        full + np.uint64(offset & 0xFFFFFFFF), full + np.uint64(offset >> 32)], axis=1)
+    words = philox4x32_10(counter, (seed & 0xFFFFFFFF, seed >> 32)).reshape(-1)[:n]
+    return words >= np.uint32(int(p * 4294967296.0))
+
+
+def dropout_f32(x, p: float, seed: int, offset: int = 0) -> np.ndarray:
+    """x * fp32(1 / (1 - p)) where kept, 0 elsewhere: one rounding, so bit for bit what fp32 arithmetic gives."""
+    x = np.asarray(x, dtype=np.float32)
+    keep = dropout_keep(x.size, p, seed, offset).reshape(x.shape)
+    scale = np.float32(1.0 / (1.0 - p)) if p < 1.0 else np.float32(0.0)
+    with np.errstate(invalid="ignore", over="ignore"):
+        return np.where(keep, x * scale, np.float32(0.0))
+
+
+# ------------------------------------------------------------ 8-bit product
+def quantize_rows(x):
+    """(q, scale) of fp32 rows: scale = fp32(max|x| / 127), q = x / scale in
+    fp64, to the nearest integer, ties to even; a row that is not finite has
+    scale NaN and q = 0."""
+    x = np.asarray(x, dtype=np.float32)
+    peak = np.abs(x).max(axis=1, initial=np.float32(0.0))
+    with np.errstate(invalid="ignore"):
+        scale = np.where(np.isfinite(peak), peak / np.float32(127.0), np.float32(np.nan)).astype(np.float32)
+    usable = np.isfinite(scale) & (scale > 0)
+    s = np.where(usable, scale, np.float32(1.0)).astype(np.float64)
+    v = np.where(usable[:, None], x, np.float32(0.0)).astype(np.float64) / s[:, None]
+    return np.clip(np.rint(v), -127, 127).astype(np.int8), scale
+
+
+def gemm_i8_f64(a, w, a_scale, w_scale, bias=None, relu=False):
+    """(value, bound) of a_scale w_scale (a . w^T) + bias.  The integer sum is
+    exact; fp32 rounds it, the product of the scales and their product (3 half
+    steps) and the sum with the bias (1): 3u |product| + u |value|, and a scale
+    that underflows rounds by an absolute 2^-150."""
+    acc = np.asarray(a, dtype=np.float64) @ np.asarray(w, dtype=np.float64).T
+    scale = np.asarray(a_scale, dtype=np.float64)[:, None] * np.asarray(w_scale, dtype=np.float64)[None, :]
+    product = acc * scale
+    value = product if bias is None else product + np.asarray(bias, dtype=np.float64)[None, :]
+    u = 2.0 ** -24
+    bound = (3.001 * u * np.abs(product) + u * np.abs(value) + (np.abs(acc) + 1) * 2.0 ** -150) * 1.001
+    return (np.maximum(value, 0.0) if relu else value), bound
