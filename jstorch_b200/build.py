@@ -35,8 +35,8 @@ NVFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler"
            "--expt-relaxed-constexpr", "-DNDEBUG", f"-I{INCLUDE}"] + ARCH
 
 GEMM_SOURCES = ["gemm_api.cu", "gemm_ffma.cu", "gemm_tc.cu", "splitk.cu", "conv.cu", "gru.cu", "hostio.cu", "profile.cu",
-                "dropout.cu", "scan.cu", "quant.cu"]
-GEMM_HEADERS = ["gemm_internal.h", "ptx.cuh"]
+                "dropout.cu", "scan.cu", "quant.cu", "gemm_i8.cu"]
+GEMM_HEADERS = ["gemm_internal.h", "gemm_i8.h", "ptx.cuh"]
 GEMM_LIB = PKG / "libjstorch_gemm.so"
 
 

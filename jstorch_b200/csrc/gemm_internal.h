@@ -57,6 +57,9 @@ inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 bl
 // JST_OK when the current device is one this library runs on (sets it up once).
 int require_device();
 
+// SMs of the current device.
+int sm_count();
+
 // Whether [a, a + na) and [b, b + nb) (bytes) have a byte in common.
 inline bool ranges_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);

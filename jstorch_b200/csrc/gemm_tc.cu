@@ -1035,8 +1035,8 @@ static int launch_persist(const CUtensorMap& a_hi, const CUtensorMap& a_lo, cons
     return JST_OK;
 }
 
-// SMs of the current device (the persistent kernel's grid).
-static int sm_count() {
+// SMs of the current device (the persistent kernels' grid).
+int sm_count() {
     static std::atomic<int> cached[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {

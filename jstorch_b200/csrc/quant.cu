@@ -7,7 +7,9 @@
 #include <cstdint>
 
 #include "../../include/jstorch_quant.h"
+#include "gemm_i8.h"
 #include "gemm_internal.h"
+#include "ptx.cuh"
 
 namespace jst {
 namespace {
@@ -29,6 +31,14 @@ __device__ __forceinline__ int quantize(float x, float s, float inv) {
 // maximum finds the peak and tells a row that is not finite.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+__device__ __forceinline__ float row_scale(uint32_t peak) {
+    return peak < 0x7f800000u ? __fdiv_rn(__uint_as_float(peak), 127.0f) : __uint_as_float(0x7fffffffu);
+}
+// 1 / s, or 0 where the row quantises to zeros (s is 0 or NaN).
+__device__ __forceinline__ float row_inverse(float s) { return s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f; }
+
+__device__ __forceinline__ int quantize_in(float x, float s, float inv) { return inv > 0.0f ? quantize(x, s, inv) : 0; }
+
 constexpr int kQuantThreads = 256;
 
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const float* __restrict__ x, int64_t ldx,
@@ -43,80 +53,163 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const floa
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
     for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, part[w]);
-    const bool finite = m < 0x7f800000u;
-    const float s = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(0x7fffffffu);
+    const float s = row_scale(m), inv = row_inverse(s);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
-    const bool zero = !finite || s == 0.0f;
-    const float inv = zero ? 0.0f : __fdiv_rn(1.0f, s);
-    for (int k = threadIdx.x; k < cols; k += kQuantThreads) out[k] = zero ? (int8_t)0 : (int8_t)quantize(row[k], s, inv);
+    for (int k = threadIdx.x; k < cols; k += kQuantThreads) out[k] = (int8_t)quantize_in(row[k], s, inv);
 }
 
-struct I8Args {
-    int M, N, K;
-    const int8_t* A; int64_t lda;
-    const int8_t* B; int64_t ldb;
-    const float* a_scale;
-    const float* b_scale;
-    const float* bias;
-    int relu;
-    float* C; int64_t ldc;
+// ------------------------------------------------------------ a few tokens
+// C[m, n] for MT <= 8 tokens.  A warp takes kChannels rows of the weight and
+// walks along K, 16 bytes a lane and row: one 16-byte piece of a token from
+// shared memory meets kChannels pieces of the weight, 4 dp4a each.  The
+// lanes' sums meet in one integer reduction, exact in any order.
+// Bound by the weight's bytes; each is read once.
+// The tokens are held in shared memory kSegment values of K at a time.  FUSED:
+// they come as fp32 rows and every block quantises them itself.
+// ALIGN: 16 when the weight's rows are 16-byte aligned.  Otherwise 1: a lane
+// reads the aligned 4-byte words that hold its 16 bytes and shifts; a word that
+// holds a byte of the row does not leave the memory block that the row is in.
+constexpr int kFewThreads = 256;
+constexpr int kChannels = 4;
+constexpr int kSegment = 8192;
+
+struct FewArgs {
+    I8Args p;        // FUSED: A and a_scale are unused
+    const float* x;  // FUSED: [M][K] fp32
+    int64_t ldx;
 };
 
-__device__ __forceinline__ float finish(int acc, float sa, float sb, bool has_bias, float bias, int relu) {
-    float v = __fmul_rn(__int2float_rn(acc), __fmul_rn(sa, sb));
-    if (has_bias) v = __fadd_rn(v, bias);
-    return relu ? fmaxf(v, 0.0f) : v;
+template <int ALIGN>
+__device__ __forceinline__ int4 load16(const int8_t* w) {
+    if (ALIGN == 16) return __ldg(reinterpret_cast<const int4*>(w));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(w);
+    const uint32_t* word = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+    const uint32_t shift = (uint32_t)(at & 3) * 8;
+    uint32_t v[5];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __ldg(word + i);
+    v[4] = shift ? __ldg(word + 4) : 0u;
+    return make_int4((int)__funnelshift_r(v[0], v[1], shift), (int)__funnelshift_r(v[1], v[2], shift),
+                     (int)__funnelshift_r(v[2], v[3], shift), (int)__funnelshift_r(v[3], v[4], shift));
 }
 
-// Any sizes, any addresses: a block of 256 threads computes 64 x 64 outputs
-// from 64-byte k-slabs in shared memory, 4 x 4 outputs a thread with dp4a.
-__global__ void __launch_bounds__(256) gemm_i8_simt_kernel(const I8Args p) {
-    constexpr int T = 64, BK = 64, LD = BK / 4 + 1;
-    __shared__ int as[T][LD], bs[T][LD];
-    const int m0 = blockIdx.y * T, n0 = blockIdx.x * T;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += BK) {
-        for (int i = threadIdx.x; i < T * BK / 4; i += 256) {
-            const int r = i / (BK / 4), w = i % (BK / 4), k = k0 + 4 * w;
-            uint32_t va = 0, vb = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (k + j >= p.K) continue;
-                if (m0 + r < p.M) va |= (uint32_t)(uint8_t)p.A[(int64_t)(m0 + r) * p.lda + k + j] << (8 * j);
-                if (n0 + r < p.N) vb |= (uint32_t)(uint8_t)p.B[(int64_t)(n0 + r) * p.ldb + k + j] << (8 * j);
-            }
-            as[r][w] = (int)va;
-            bs[r][w] = (int)vb;
+__device__ __forceinline__ int dot16(int4 a, int4 b, int c) {
+    return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, c))));
+}
+
+template <int MT, int ALIGN, bool FUSED>
+__global__ void __launch_bounds__(kFewThreads) gemm_i8_few_kernel(const FewArgs f) {
+    extern __shared__ __align__(16) int8_t tokens[];  // [MT][seg], seg a multiple of 16
+    __shared__ uint32_t part[MT][kFewThreads / 32];
+    __shared__ float scales[MT], inverses[MT];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const I8Args& p = f.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n0 = (blockIdx.x * (kFewThreads / 32) + warp) * kChannels;
+    if (FUSED) {
+        for (int m = 0; m < MT; ++m) {
+            uint32_t peak = 0;
+            if (m < p.M)
+                for (int k = threadIdx.x; k < p.K; k += kFewThreads) peak = max(peak, abs_bits(__ldg(f.x + m * f.ldx + k)));
+            peak = __reduce_max_sync(0xffffffffu, peak);
+            if (lane == 0) part[m][warp] = peak;
         }
         __syncthreads();
-#pragma unroll 4
-        for (int w = 0; w < BK / 4; ++w) {
-            int a[4], b[4];
+        if (threadIdx.x < MT) {
+            uint32_t peak = 0;
+            for (int w = 0; w < kFewThreads / 32; ++w) peak = max(peak, part[threadIdx.x][w]);
+            scales[threadIdx.x] = row_scale(peak);
+            inverses[threadIdx.x] = row_inverse(scales[threadIdx.x]);
+        }
+        __syncthreads();
+    }
+    int acc[kChannels][MT] = {};
+    for (int k0 = 0; k0 < p.K; k0 += kSegment) {
+        const int len = min(kSegment, p.K - k0), seg = (len + 15) & ~15;
+        for (int i = threadIdx.x * 4; i < MT * seg; i += kFewThreads * 4) {  // seg is a multiple of 4
+            const int m = i / seg, k = i - m * seg;
+            uint32_t v = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = as[ty * 4 + i][w];
-                b[i] = bs[tx + 16 * i][w];
+            for (int j = 0; j < 4; ++j)
+                if (m < p.M && k + j < len) {
+                    const int q = FUSED ? quantize_in(__ldg(f.x + m * f.ldx + k0 + k + j), scales[m], inverses[m])
+                                        : p.A[m * p.lda + k0 + k + j];
+                    v |= (uint32_t)(uint8_t)q << (8 * j);
+                }
+            *reinterpret_cast<uint32_t*>(tokens + i) = v;
+        }
+        __syncthreads();
+        if (n0 < p.N) {
+            const int8_t* row[kChannels];
+#pragma unroll
+            for (int c = 0; c < kChannels; ++c) row[c] = p.B + (int64_t)min(n0 + c, p.N - 1) * p.ldb + k0;
+            const int whole = len & ~15;
+#pragma unroll 2
+            for (int k = lane * 16; k < whole; k += 512) {
+                int4 w[kChannels];
+#pragma unroll
+                for (int c = 0; c < kChannels; ++c) w[c] = load16<ALIGN>(row[c] + k);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const int4 t = *reinterpret_cast<const int4*>(tokens + m * seg + k);
+#pragma unroll
+                    for (int c = 0; c < kChannels; ++c) acc[c][m] = dot16(w[c], t, acc[c][m]);
+                }
             }
+            if (lane < len - whole)  // the row's last bytes, one a lane
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int c = 0; c < kChannels; ++c)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[i], b[j], acc[i][j]);
+                    for (int m = 0; m < MT; ++m) acc[c][m] += (int)row[c][whole + lane] * (int)tokens[m * seg + whole + lane];
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int m = m0 + ty * 4 + i;
-        if (m >= p.M) continue;
+    for (int c = 0; c < kChannels; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + tx + 16 * j;
-            if (n < p.N)
-                p.C[(int64_t)m * p.ldc + n] =
-                    finish(acc[i][j], p.a_scale[m], p.b_scale[n], p.bias != nullptr, p.bias ? p.bias[n] : 0.0f, p.relu);
+        for (int m = 0; m < MT; ++m) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[c][m]);
+            const int n = n0 + c;
+            if (lane == (c * MT + m) % 32 && n < p.N && m < p.M)
+                p.C[m * p.ldc + n] = i8_finish(sum, FUSED ? scales[m] : p.a_scale[m], p.b_scale[n], p.bias != nullptr,
+                                               p.bias ? p.bias[n] : 0.0f, p.relu);
         }
-    }
+}
+
+template <int MT, int ALIGN, bool FUSED>
+int launch_few(const FewArgs& f, cudaStream_t s) {
+    const unsigned grid = (unsigned)((f.p.N + kFewThreads / 32 * kChannels - 1) / (kFewThreads / 32 * kChannels));
+    const size_t smem = (size_t)MT * ((std::min(f.p.K, kSegment) + 15) & ~15);
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(gemm_i8_few_kernel<MT, ALIGN, FUSED>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, MT * kSegment) != cudaSuccess)
+        return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(gemm_i8_few_kernel) failed");
+    ProfScope prof(s, KID_GEMM_I8);
+    if (launch_dependent(gemm_i8_few_kernel<MT, ALIGN, FUSED>, dim3(grid), dim3(kFewThreads), smem, s, f) != cudaSuccess)
+        return set_status(JST_ERR_CUDA, "gemm_i8_few_kernel launch failed");
+    return JST_OK;
+}
+
+template <bool FUSED>
+int run_few(const FewArgs& f, cudaStream_t s) {
+    const bool al = (reinterpret_cast<uintptr_t>(f.p.B) & 15) == 0 && (f.p.N == 1 || (f.p.ldb & 15) == 0);
+    if (f.p.M == 1) return al ? launch_few<1, 16, FUSED>(f, s) : launch_few<1, 1, FUSED>(f, s);
+    if (f.p.M == 2) return al ? launch_few<2, 16, FUSED>(f, s) : launch_few<2, 1, FUSED>(f, s);
+    if (f.p.M <= 4) return al ? launch_few<4, 16, FUSED>(f, s) : launch_few<4, 1, FUSED>(f, s);
+    return al ? launch_few<8, 16, FUSED>(f, s) : launch_few<8, 1, FUSED>(f, s);
+}
+
+// K == 0: every sum is 0.
+__global__ void empty_sums_kernel(const I8Args p) {
+    for (int64_t m = blockIdx.y; m < p.M; m += gridDim.y)
+        for (int64_t n = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; n < p.N; n += (int64_t)gridDim.x * blockDim.x)
+            p.C[m * p.ldc + n] = i8_finish(0, 0.0f, 0.0f, p.bias != nullptr, p.bias ? p.bias[n] : 0.0f, p.relu);
+}
+
+int run_empty(const I8Args& p, cudaStream_t s) {
+    ProfScope prof(s, KID_GEMM_I8);
+    empty_sums_kernel<<<dim3((unsigned)std::min((p.N + 255) / 256, 1024), (unsigned)std::min(p.M, 1024)), 256, 0, s>>>(p);
+    return JST_OK;
 }
 
 int launched(const char* what) {
@@ -157,12 +250,16 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     return JST_OK;
 }
 
+// Up to kFew tokens the product is a read of the weight, and dp4a keeps up
+// with it; from there on the tensor cores' work a byte of weight is free.
+constexpr int kFew = 8;
+// Up to so many values every block of the product quantises the tokens itself;
+// more are quantised once, by a launch of their own.
+constexpr int64_t kFusedValues = 16384;
+
 int run_gemm_i8(const I8Args& p, cudaStream_t s) {
-    {
-        ProfScope prof(s, KID_GEMM_I8);
-        gemm_i8_simt_kernel<<<dim3((p.N + 63) / 64, (p.M + 63) / 64), 256, 0, s>>>(p);
-    }
-    return launched("gemm_i8 launch failed");
+    const int rc = p.K == 0 ? run_empty(p, s) : p.M <= kFew ? run_few<false>({p, nullptr, 0}, s) : gemm_i8_tc_run(p, s);
+    return rc ? rc : launched("gemm_i8 launch failed");
 }
 
 }  // namespace
@@ -211,6 +308,12 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
     if (rc) return rc;
     if (M == 0 || N == 0) return set_status(JST_OK, nullptr);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    I8Args p{M, N, K, nullptr, 0, w, ldw, nullptr, w_scale, (epilogue & JST_EPI_BIAS) ? bias : nullptr,
+             (epilogue & JST_EPI_RELU) ? 1 : 0, y, ldy};
+    if (K == 0 || (M <= kFew && (int64_t)M * K <= kFusedValues)) {
+        rc = K == 0 ? run_empty(p, s) : run_few<true>({p, x, ldx}, s);
+        return rc ? rc : launched("linear_i8 launch failed");
+    }
     const int64_t ldq = ((int64_t)K + 15) / 16 * 16;
     const size_t scale_bytes = ((size_t)M * 4 + 255) & ~size_t(255);
     void* ws = nullptr;
@@ -220,8 +323,9 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
     int8_t* q = static_cast<int8_t*>(ws) + scale_bytes;
     rc = run_quantize(x, ldx, M, K, q, ldq, scale, s);
     if (!rc) {
-        I8Args p{M, N, K, q, ldq, w, ldw, scale, w_scale, (epilogue & JST_EPI_BIAS) ? bias : nullptr,
-                 (epilogue & JST_EPI_RELU) ? 1 : 0, y, ldy};
+        p.A = q;
+        p.lda = ldq;
+        p.a_scale = scale;
         rc = run_gemm_i8(p, s);
     }
     const int frc = workspace_free(ws, s);
