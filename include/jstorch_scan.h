@@ -22,6 +22,7 @@ enum { JST_SCAN_TANH = 0, JST_SCAN_IDENTITY = 1 };
  *   z = sigmoid(a)    n = tanh(c) or c    h_t = z * h_{t-1} + (1 - z) * n
  *   gates    row (t, b) at gates + (t * batch + b) * ld_gates: a in columns
  *            [0, hidden), c in [hidden, 2 * hidden); ld_gates >= 2 * hidden
+ *            (every pitch is below 2^24)
  *   h0       [batch][hidden] or NULL (zeros)
  *   lengths  [batch] int32 on the device, or NULL (every sequence has seq
  *            steps).  Sequence b has min(max(lengths[b], 0), seq) steps, the

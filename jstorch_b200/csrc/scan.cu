@@ -11,6 +11,14 @@
 //            the last one),  A = z_t,  B = z_t dout_t
 // A step outside its sequence is A = 1, B = 0, chosen by comparison, so what
 // the gates hold there (infinities and NaN too) does not matter.
+//
+// Bytes a step and channel: forward 8 read, 4 written; backward 16 read, 8
+// written; nothing but the outputs is kept for the backward pass, which makes
+// the gates again.  Reached on a B200 (tanh): 2048 x 16 x 1024 forward 81 us
+// (5.0 TB/s, 0.76 of the measured copy rate), backward 143 us (5.6 TB/s, 0.86);
+// 65536 x 1 x 1024, identity, 188 us (4.3 TB/s) and 312 us (5.2 TB/s), where
+// one tile's rounds follow each other.  Forward, what is left is issue slots:
+// 40 instructions for 12 bytes.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -18,6 +26,7 @@
 
 #include "../../include/jstorch_scan.h"
 #include "gemm_internal.h"
+#include "ptx.cuh"
 
 namespace jst {
 namespace {
@@ -34,97 +43,561 @@ struct ScanArgs {
     float* dgates; int64_t ld_dgates;
     float* dh0;
     int seq, batch, hidden, reverse;
+    uint32_t* err;
 };
 
-// sigmoid(a) and 1 - sigmoid(a) from one exponential of -|a|: neither loses
-// digits where it is small.
-__device__ __forceinline__ void gate(float a, float& z, float& rest) {
-    const float e = expf(-fabsf(a));
-    const float big = __fdividef(1.0f, 1.0f + e), small = e * big;
-    z = a >= 0.0f ? big : small;
-    rest = a >= 0.0f ? small : big;
+// V adjacent channels of one step.  Pairs go through the two-wide fp32
+// instructions: with a few loads, one exponential and one reciprocal a gate the
+// issue slots are what limits an SM here, and a pair takes one slot for both.
+template <int V>
+struct F {
+    float v[V];
+};
+__device__ __forceinline__ uint64_t pack(const F<2>& a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+    return r;
 }
-
-template <bool TANH>
-__device__ __forceinline__ float candidate(float c) {
-    return TANH ? tanhf(c) : c;
+__device__ __forceinline__ F<2> unpack(uint64_t a) {
+    F<2> r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(a));
+    return r;
 }
-
-// One thread per channel walks the time axis, K steps' loads at a time.
-constexpr int kSerialThreads = 128;
-constexpr int kSerialSteps = 8;
-
-template <bool TANH>
-__global__ void __launch_bounds__(kSerialThreads) scan_forward_serial_kernel(const ScanArgs p) {
-    const int64_t channels = (int64_t)p.batch * p.hidden;
-    const int64_t ch = blockIdx.x * (int64_t)kSerialThreads + threadIdx.x;
-    if (ch >= channels) return;
-    const int b = (int)(ch / p.hidden), j = (int)(ch - (int64_t)b * p.hidden);
-    const int len = p.lengths ? min(max(p.lengths[b], 0), p.seq) : p.seq;
-    const int64_t step_g = (int64_t)p.batch * p.ld_gates, step_o = (int64_t)p.batch * p.ld_out;
-    const float* g = p.gates + b * p.ld_gates + j;
-    float* o = p.out + b * p.ld_out + j;
-    float h = p.h0 ? p.h0[ch] : 0.0f;
-    for (int s0 = 0; s0 < p.seq; s0 += kSerialSteps) {
-        float a[kSerialSteps], c[kSerialSteps];
+template <int V>
+__device__ __forceinline__ F<V> all(float x) {
+    F<V> r;
 #pragma unroll
-        for (int i = 0; i < kSerialSteps; ++i) {
-            const int s = s0 + i, t = p.reverse ? p.seq - 1 - s : s;
-            const bool in = s < p.seq && t < len;
-            a[i] = in ? g[t * step_g] : 0.0f;
-            c[i] = in ? g[t * step_g + p.hidden] : 0.0f;
+    for (int i = 0; i < V; ++i) r.v[i] = x;
+    return r;
+}
+template <int V>
+__device__ __forceinline__ F<V> fma(const F<V>& a, const F<V>& b, const F<V>& c) {
+    if constexpr (V == 2) {
+        uint64_t r;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack(a)), "l"(pack(b)), "l"(pack(c)));
+        return unpack(r);
+    } else {
+        return {fmaf(a.v[0], b.v[0], c.v[0])};
+    }
+}
+template <int V>
+__device__ __forceinline__ F<V> operator*(const F<V>& a, const F<V>& b) {
+    if constexpr (V == 2) {
+        uint64_t r;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack(a)), "l"(pack(b)));
+        return unpack(r);
+    } else {
+        return {__fmul_rn(a.v[0], b.v[0])};
+    }
+}
+template <int V>
+__device__ __forceinline__ F<V> operator+(const F<V>& a, const F<V>& b) {
+    if constexpr (V == 2) {
+        uint64_t r;
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack(a)), "l"(pack(b)));
+        return unpack(r);
+    } else {
+        return {__fadd_rn(a.v[0], b.v[0])};
+    }
+}
+template <int V>
+__device__ __forceinline__ F<V> operator-(const F<V>& a) {  // folds into the operation that takes it
+    F<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = -a.v[i];
+    return r;
+}
+
+// exp(-x) as 2^(-x log2 e), |x| <= 127: the rounding error of that product (and
+// of log2 e) is found by a fused multiply-add and put back to first order, so
+// what is left is the 2^-22 of the power and a rounding.  Results below 2^-126
+// flush to 0.
+template <int V>
+__device__ __forceinline__ F<V> exp_minus(const F<V>& x) {
+    const float log2e = 1.44269502162933349609375f, log2e_rest = 1.92596299112661746887e-8f;
+    const F<V> t = x * all<V>(-log2e);
+    F<V> r = fma(x, all<V>(-log2e), -t);
+    r = fma(x, all<V>(-log2e_rest), r) * all<V>(0.693147180559945309f);
+    F<V> e;
+#pragma unroll
+    for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v[i]) : "f"(t.v[i]));
+    return fma(e, r, e);
+}
+template <int V>
+__device__ __forceinline__ F<V> reciprocal(const F<V>& x) {
+    F<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v[i]) : "f"(x.v[i]));
+    return r;
+}
+// Clamps that a NaN passes.
+__device__ __forceinline__ float at_least(float x, float lo) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float at_most(float x, float hi) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(hi));
+    return r;
+}
+
+// z = 1 / (1 + e) and 1 - z = e z with e = exp(-a): neither loses digits where
+// it is small.  a is kept within [-87, 127], where e is a number and z is
+// positive: below, z is held at 2^-126 (1.65e-38), which a state's share of
+// the next one cannot show beside anything but 0.
+template <int V>
+__device__ __forceinline__ void gate(const F<V>& a, F<V>& z, F<V>& rest) {
+    F<V> x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) x.v[i] = at_most(at_least(a.v[i], -87.0f), 127.0f);
+    const F<V> e = exp_minus(x);
+    z = reciprocal(e + all<V>(1.0f));
+    rest = e * z;
+}
+
+// tanh(c) = (1 - t) / (1 + t) of |c| with t = exp(-2 |c|), and below 0.6, where
+// 1 - t would lose digits, c + c^3 P(c^2) with P of degree 4 fitted to the
+// relative error (0.05 of 2^-24).
+template <bool TANH, int V>
+__device__ __forceinline__ F<V> candidate(const F<V>& c) {
+    if constexpr (!TANH) return c;
+    F<V> x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) x.v[i] = at_most(fabsf(c.v[i]), 60.0f);
+    const F<V> t = exp_minus(x + x);
+    const F<V> far = (all<V>(1.0f) + -t) * reciprocal(t + all<V>(1.0f));
+    const F<V> q = c * c;
+    F<V> p = fma(q, all<V>(-0.005895157810300589f), all<V>(0.020795971155166626f));
+    p = fma(p, q, all<V>(-0.053783830255270004f));
+    p = fma(p, q, all<V>(0.13331924378871918f));
+    p = fma(p, q, all<V>(-0.33333298563957214f));
+    const F<V> near = fma(c * q, p, c);
+    F<V> n;
+#pragma unroll
+    for (int i = 0; i < V; ++i) n.v[i] = fabsf(c.v[i]) < 0.6f ? near.v[i] : copysignf(far.v[i], c.v[i]);
+    return n;
+}
+
+// A product of z in (0, 1) underflows to 0 after some hundred steps, and 0 times
+// an infinite state would be NaN where step by step it stays infinite: as no z
+// is 0, products are kept at 2^-149 at least (2^-149 of the state, far below a
+// rounding of what is added to it).
+constexpr float kTiny = 1.40129846432481707e-45f;
+
+template <int V>
+__device__ __forceinline__ F<V> load(const char* p) {
+    if constexpr (V == 2) {
+        const float2 x = __ldcs(reinterpret_cast<const float2*>(p));
+        return {x.x, x.y};
+    } else {
+        return {__ldcs(reinterpret_cast<const float*>(p))};
+    }
+}
+template <int V>
+__device__ __forceinline__ void store(char* p, const F<V>& x) {
+    if constexpr (V == 2) *reinterpret_cast<float2*>(p) = make_float2(x.v[0], x.v[1]);
+    else *reinterpret_cast<float*>(p) = x.v[0];
+}
+
+// Rows of one array as a warp walks them: the address of the tile's first
+// channel at the pass's first step and the bytes of a step (both the same in
+// all lanes, so steps are added in the uniform datapath), and this lane's
+// bytes behind the tile's first channel.
+struct Rows {
+    char* base;
+    int64_t step;
+    uint32_t lane;
+
+    __device__ __forceinline__ char* at(int64_t s) const { return base + s * step; }
+};
+
+// A warp's 32 * V channels and the direction of its pass.
+template <bool BWD, int V>
+struct Channels {
+    bool mine;   // this lane's channels exist
+    int64_t ch;  // its first one
+    int lo, hi;  // steps of this pass inside its sequence: [lo, hi)
+    uint32_t c;  // bytes from a row's a to its c
+    Rows gates, out, dout, dgates;  // backward: out is h of the step that comes next in this pass
+
+    __device__ __forceinline__ Rows rows(const ScanArgs& p, const float* x, int64_t ld, bool down, int64_t tile,
+                                         int b, int j) const {
+        const int b0 = (int)(tile / p.hidden), j0 = (int)(tile - (int64_t)b0 * p.hidden);
+        Rows r;
+        r.step = (down ? -4 : 4) * (p.batch * ld);
+        r.base = const_cast<char*>(reinterpret_cast<const char*>(x + ((down ? p.seq - 1 : 0) * (int64_t)p.batch + b0) * ld + j0));
+        r.lane = (uint32_t)(((b - b0) * ld + (j - j0)) * 4);
+        return r;
+    }
+    // tile: the warp's first channel, the same in every lane
+    __device__ __forceinline__ Channels(const ScanArgs& p, int64_t tile, int lane) {
+        ch = tile + lane * V;
+        const int64_t channels = (int64_t)p.batch * p.hidden;
+        mine = ch < channels;
+        const int64_t at = mine ? ch : channels - V;  // a lane past the end reads and writes nothing
+        const int b = (int)(at / p.hidden), j = (int)(at - (int64_t)b * p.hidden);
+        const int len = !mine ? 0 : p.lengths ? min(max(p.lengths[b], 0), p.seq) : p.seq;
+        const bool down = BWD ? !p.reverse : p.reverse != 0;  // from the last step to the first
+        lo = down ? p.seq - len : 0;
+        hi = lo + len;
+        c = (uint32_t)p.hidden * 4;
+        gates = rows(p, p.gates, p.ld_gates, down, tile, b, j);
+        if (BWD) {
+            out = rows(p, p.out_in, p.ld_out, down, tile, b, j);
+            out.base += out.step;
+            dout = rows(p, p.dout, p.ld_dout, down, tile, b, j);
+            dgates = rows(p, p.dgates, p.ld_dgates, down, tile, b, j);
+        } else {
+            out = rows(p, p.out, p.ld_out, down, tile, b, j);
         }
+    }
+    __device__ __forceinline__ F<V> state(const float* p) const {
+        F<V> r;
 #pragma unroll
-        for (int i = 0; i < kSerialSteps; ++i) {
-            const int s = s0 + i, t = p.reverse ? p.seq - 1 - s : s;
-            if (s >= p.seq) break;
-            if (t < len) {
-                float z, rest;
-                gate(a[i], z, rest);
-                h = fmaf(z, h, rest * candidate<TANH>(c[i]));
+        for (int i = 0; i < V; ++i) r.v[i] = mine && p ? p[ch + i] : 0.0f;
+        return r;
+    }
+    __device__ __forceinline__ void set_state(float* p, const F<V>& x) const {
+        if (mine && p)
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[ch + i] = x.v[i];
+    }
+    // whether steps [s, s + n) are inside every lane's sequence
+    __device__ __forceinline__ bool whole(int64_t s, int n) const {
+        return __all_sync(0xffffffffu, s >= lo && s + n <= hi);
+    }
+    __device__ __forceinline__ bool in(int64_t s) const { return s >= lo && s < hi; }
+};
+
+// K steps of a lane's channels as they come from memory.
+template <bool BWD, int V, int K>
+struct Raw {
+    F<V> a[K], c[K], h[BWD ? K : 1], d[BWD ? K : 1];
+
+    template <bool ALL, bool DOUT>
+    __device__ __forceinline__ void fetch_part(const Channels<BWD, V>& w, const F<V>& h_first, int64_t s0) {
+        const char *g = w.gates.at(s0), *o = BWD ? w.out.at(s0) : nullptr, *d0 = BWD ? w.dout.at(s0) : nullptr;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const bool in = ALL || w.in(s0 + i);
+            a[i] = in ? load<V>(g + w.gates.lane) : all<V>(0.0f);
+            c[i] = in ? load<V>(g + w.c + w.gates.lane) : all<V>(0.0f);
+            g += w.gates.step;
+            if (BWD) {
+                // the last step inside the sequence is the one that started from h0
+                h[i] = !in ? all<V>(0.0f) : !ALL && s0 + i + 1 == w.hi ? h_first : load<V>(o + w.out.lane);
+                d[i] = DOUT && in ? load<V>(d0 + w.dout.lane) : all<V>(0.0f);
+                o += w.out.step;
+                d0 += w.dout.step;
             }
-            o[t * step_o] = t < len ? h : 0.0f;
         }
     }
-    if (p.h_n) p.h_n[ch] = h;
+    __device__ __forceinline__ void fetch(const ScanArgs& p, const Channels<BWD, V>& w, const F<V>& h_first, int64_t s0) {
+        if (w.whole(s0, BWD ? K + 1 : K)) {
+            if (!BWD || p.dout) fetch_part<true, BWD>(w, h_first, s0);
+            else fetch_part<true, false>(w, h_first, s0);
+        } else {
+            if (!BWD || p.dout) fetch_part<false, BWD>(w, h_first, s0);
+            else fetch_part<false, false>(w, h_first, s0);
+        }
+    }
+};
+
+// What the outputs of K steps need once the state before them is known:
+// forward z and (1 - z) n; backward z, dout, and da and dc per unit of G.
+template <bool BWD, int V, int K>
+struct Steps {
+    F<V> z[K], add[K], fa[BWD ? K : 1], fc[BWD ? K : 1];
+
+    template <bool TANH>
+    __device__ __forceinline__ void from(const Raw<BWD, V, K>& r, const Channels<BWD, V>& w, int64_t s0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            F<V> rest;
+            gate(r.a[i], z[i], rest);
+            const F<V> n = candidate<TANH>(r.c[i]);
+            if (BWD) {
+                fa[i] = (r.h[i] + -n) * (z[i] * rest);
+                fc[i] = TANH ? rest * fma(-n, n, all<V>(1.0f)) : rest;
+                add[i] = r.d[i];
+            } else {
+                add[i] = rest * n;
+            }
+        }
+        if (!w.whole(s0, K))
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                if (w.in(s0 + i)) continue;
+                z[i] = all<V>(1.0f);  // the state passes over the step
+                add[i] = all<V>(0.0f);
+            }
+    }
+    // the steps as one pair (A, B): e -> A e + B
+    __device__ __forceinline__ void fold(F<V>& A, F<V>& B) const {
+        A = z[0];
+        B = BWD ? z[0] * add[0] : add[0];
+#pragma unroll
+        for (int i = 1; i < K; ++i) {
+            B = BWD ? z[i] * (B + add[i]) : fma(z[i], B, add[i]);
+            A = A * z[i];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) A.v[v] = fmaxf(A.v[v], kTiny);
+    }
+    template <bool ALL>
+    __device__ __forceinline__ F<V> finish_part(F<V> e, int seq, const Channels<BWD, V>& w, int64_t s0) const {
+        const Rows& r = BWD ? w.dgates : w.out;
+        char* o = r.at(s0);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const bool in = ALL || w.in(s0 + i), exists = ALL || (w.mine && s0 + i < seq);
+            if (BWD) {
+                const F<V> G = e + add[i];
+                const F<V> da = G * fa[i], dc = G * fc[i];
+                if (exists) {
+                    store(o + r.lane, in ? da : all<V>(0.0f));
+                    store(o + w.c + r.lane, in ? dc : all<V>(0.0f));
+                }
+                e = z[i] * G;
+            } else {
+                e = fma(z[i], e, add[i]);
+                if (exists) store(o + r.lane, in ? e : all<V>(0.0f));
+            }
+            o += r.step;
+        }
+        return e;
+    }
+    // the state (or what is handed back) after the K steps; writes their outputs
+    __device__ __forceinline__ F<V> finish(F<V> e, int seq, const Channels<BWD, V>& w, int64_t s0) const {
+        return w.whole(s0, K) ? finish_part<true>(e, seq, w, s0) : finish_part<false>(e, seq, w, s0);
+    }
+};
+
+// The warp's index, known to the compiler as the same in all lanes.
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+
+// ------------------------------------------------------------ short sequences
+// One lane walks its channels' time axis, K steps' loads at a time.
+constexpr int kSerialThreads = 128;
+
+template <bool BWD, bool TANH, int V, int K>
+__global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const ScanArgs p) {
+    const int64_t tile = (blockIdx.x * (int64_t)(kSerialThreads / 32) + warp_index()) * 32 * V;
+    if (tile >= (int64_t)p.batch * p.hidden) return;
+    const Channels<BWD, V> w(p, tile, threadIdx.x & 31);
+    const F<V> h_first = w.state(p.h0);
+    F<V> e = BWD ? w.state(p.dh_n) : h_first;
+    for (int64_t s0 = 0; s0 < p.seq; s0 += K) {
+        Raw<BWD, V, K> r;
+        r.fetch(p, w, h_first, s0);
+        Steps<BWD, V, K> st;
+        st.template from<TANH>(r, w, s0);
+        e = st.finish(e, p.seq, w, s0);
+    }
+    w.set_state(BWD ? p.dh0 : p.h_n, e);
 }
 
-template <bool TANH>
-__global__ void __launch_bounds__(kSerialThreads) scan_backward_serial_kernel(const ScanArgs p) {
+// ------------------------------------------------------------ split along time
+// A pair (A, B) stands for e -> A e + B.  K steps in a lane's registers fold
+// into one pair; applying the pairs in the order of time to the state that the
+// round starts from gives every lane the state before its own first step, and
+// a second pass over the registers gives the outputs: the data are read once.
+//   block    S warps over the same 32 * V channels (V a lane), K consecutive
+//            steps a warp: one row segment of 32 * V floats a load;
+//   cluster  C blocks over consecutive runs of S * K steps; each sends the
+//            pair of its run to the others through distributed shared memory,
+//            counted in by a barrier of the receiver (a cluster-wide barrier
+//            a round would wait for every load and store in flight);
+//   loop     until the time axis ends, C * S * K steps a round, with the next
+//            round's loads in flight while this one is folded and written.
+// Every order is fixed, so results repeat bit for bit.
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// V channels' pair in shared memory.
+template <int V>
+struct __align__(8 * V) Pair {
+    F<V> A, B;
+};
+// Store to the same place in block `rank` of the cluster; its barrier counts the bytes as they arrive.
+template <int V>
+__device__ __forceinline__ void send(Pair<V>* to, uint64_t* bar, int rank, const Pair<V>& v) {
+    uint32_t at, at_bar;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(to)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_bar) : "r"(ptx::smem_u32(bar)), "r"(rank));
+    if constexpr (V == 2)
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at),
+                     "r"(__float_as_uint(v.A.v[0])), "r"(__float_as_uint(v.A.v[1])), "r"(__float_as_uint(v.B.v[0])),
+                     "r"(__float_as_uint(v.B.v[1])), "r"(at_bar)
+                     : "memory");
+    else
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(at),
+                     "r"(__float_as_uint(v.A.v[0])), "r"(__float_as_uint(v.B.v[0])), "r"(at_bar)
+                     : "memory");
+}
+
+template <bool BWD, bool TANH, int V, int S, int K, int BLOCKS>
+__global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanArgs p, int C) {
+    __shared__ Pair<V> warps[2][S][32];   // the warps' folds, two rounds
+    __shared__ Pair<V> blocks[2][8][32];  // the folds of the cluster's blocks, two rounds
+    __shared__ uint64_t arrived[2];
+    __shared__ uint32_t gave_up;
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x % C);  // C divides the grid: the block's rank in its cluster
+    const Channels<BWD, V> w(p, (blockIdx.x / C) * (int64_t)(32 * V), lane);
+    const F<V> h_first = w.state(p.h0);
+    F<V> carry = BWD ? w.state(p.dh_n) : h_first;
+    const int64_t round_steps = (int64_t)C * S * K, my_first = (int64_t)(rank * S + warp) * K;
+    Raw<BWD, V, K> raw;
+    raw.fetch(p, w, h_first, my_first);
+    if (C > 1) {
+        if (threadIdx.x == 0) {
+            ptx::mbar_init(&arrived[0], 1);
+            ptx::mbar_init(&arrived[1], 1);
+            gave_up = 0;
+            ptx::fence_barrier_init();
+        }
+        cluster_arrive();  // every block's barriers are set up before any block sends
+        cluster_wait();
+    }
+    uint32_t round = 0;
+    for (int64_t base = 0; base < p.seq; base += round_steps, ++round) {
+        const int parity = round & 1;
+        const int64_t s0 = base + my_first;
+        if (C > 1 && threadIdx.x == 0) ptx::mbar_arrive_expect_tx(&arrived[parity], (uint32_t)(C * 32 * sizeof(Pair<V>)));
+        Steps<BWD, V, K> st;
+        st.template from<TANH>(raw, w, s0);
+        {
+            Pair<V> mine;
+            st.fold(mine.A, mine.B);
+            warps[parity][warp][lane] = mine;
+        }
+        if (base + round_steps < p.seq) raw.fetch(p, w, h_first, s0 + round_steps);
+        // One barrier a round: a warp writes these places again two rounds on,
+        // past the next barrier, which every warp reaches after reading them.
+        __syncthreads();
+        F<V> e = carry;  // the state before this block's run, then before this warp's
+        if (C > 1) {
+            if (warp == 0) {
+                Pair<V> run = warps[parity][0][lane];
+#pragma unroll
+                for (int q = 1; q < S; ++q) {
+                    const Pair<V> f = warps[parity][q][lane];
+                    run.B = fma(f.A, run.B, f.B);
+                    run.A = f.A * run.A;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) run.A.v[v] = fmaxf(run.A.v[v], kTiny);
+                }
+                // A block is two rounds ahead of another's reads of these places
+                // only after that other has sent the round between: it has read them.
+                for (int q = 0; q < C; ++q) send(&blocks[parity][rank][lane], &arrived[parity], q, run);
+            }
+            ptx::mbar_wait(&arrived[parity], (round >> 1) & 1, &gave_up);
+            for (int q = 0; q < C; ++q) {
+                if (q == rank) e = carry;
+                const Pair<V> f = blocks[parity][q][lane];
+                carry = fma(f.A, carry, f.B);
+            }
+#pragma unroll
+            for (int q = 0; q < S - 1; ++q) {
+                if (q >= warp) break;
+                const Pair<V> f = warps[parity][q][lane];
+                e = fma(f.A, e, f.B);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                if (q == warp) e = carry;
+                const Pair<V> f = warps[parity][q][lane];
+                carry = fma(f.A, carry, f.B);
+            }
+        }
+        st.finish(e, p.seq, w, s0);
+    }
+    if (rank == 0 && warp == 0) w.set_state(BWD ? p.dh0 : p.h_n, carry);
+    if (C > 1) {
+        if (threadIdx.x == 0 && gave_up) atomicOr(p.err, gave_up);
+        cluster_arrive();  // nobody leaves while another could still send to it
+        cluster_wait();
+    }
+}
+
+template <bool BWD, bool TANH, int V, int S, int K, int BLOCKS>
+int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
+    const int64_t tiles = ((int64_t)p.batch * p.hidden + 32 * V - 1) / (32 * V);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * C));
+    cfg.blockDim = dim3(32 * S);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    ProfScope prof(s, KID_SCAN);
+    return cudaLaunchKernelEx(&cfg, scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>, p, C) == cudaSuccess
+               ? JST_OK
+               : set_status(JST_ERR_CUDA, "scan launch failed");
+}
+
+// Which kernel, and how the time axis is split.  Times in us, tanh, forward
+// and backward, on a B200 (tile: the 32 * V channels of a warp).
+//   * A few steps, or enough channels to fill the SMs by themselves: one lane
+//     walks the axis (4 x 64 x 1024 [seq x batch x hidden]: 2.7 / 3.5, split
+//     over warps 5.7 / 8.8; 16 x 64 x 1024: 6.2 / 8.0, split 6.1 / 10.1;
+//     128 x 256 x 1024: 71 / 136, split 84 / 150).
+//   * Many tiles of a short axis: small blocks, of which many fit an SM
+//     (64 x 64 x 1024: 11.9 / 18.3; in blocks of 8 warps x 8 steps 15.1 / 24.8).
+//   * Otherwise 64 steps a block and round, 8 a lane (2048 x 16 x 1024 forward
+//     81, with 4 steps a lane 100; backward 4 warps x 8 steps 143, 8 x 8 146,
+//     4 x 4 200), and where the tiles leave SMs empty, clusters that share a
+//     tile's axis: forward 2 blocks fit an SM, backward 1 (4096 x 1 x 4096:
+//     47 / 83 in clusters of 4 / 2, 94 / 122 without).
+//   * So few channels that even clusters of 8 blocks leave SMs empty: one
+//     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 188 / 312
+//     against 240 / 428 with two).
+template <bool BWD, bool TANH, int V>
+int run_scan(const ScanArgs& p, cudaStream_t s) {
+    const int64_t channels = (int64_t)p.batch * p.hidden, tiles = (channels + 32 * V - 1) / (32 * V);
+    const int sms = sm_count();
+    if (p.seq <= 16 || channels >= 131072) {
+        const int64_t grid = (tiles + kSerialThreads / 32 - 1) / (kSerialThreads / 32);
+        if (grid > 0x7fffffff) return set_status(JST_ERR_ARG, "scan: too many channels");
+        ProfScope prof(s, KID_SCAN);
+        scan_serial_kernel<BWD, TANH, V, 4><<<(unsigned)grid, kSerialThreads, 0, s>>>(p);
+        return JST_OK;
+    }
+    if (p.seq <= 64 && tiles >= 4 * sms) return launch_tiled<BWD, TANH, V, 4, 4, BWD ? 5 : 8>(p, 1, s);
+    if (BWD && V == 2 && tiles >= sms) return launch_tiled<BWD, TANH, V, 4, 8, 1>(p, 1, s);
+    constexpr int blocks_per_sm = BWD && V == 2 ? 1 : 2;
+    int C = 1;
+    while (C < 8 && tiles * C * 2 <= sms * blocks_per_sm && p.seq > C * 64) C *= 2;
+    return launch_tiled<BWD, TANH, V, 8, 8, blocks_per_sm>(p, C, s);
+}
+
+// Whether the V = 2 kernels' 8-byte accesses are aligned.
+bool pairs_ok(const ScanArgs& p) {
+    if (p.hidden & 1) return false;
+    const struct { const void* at; int64_t ld; } rows[] = {
+        {p.gates, p.ld_gates}, {p.out_in, p.ld_out}, {p.out, p.ld_out}, {p.dout, p.ld_dout}, {p.dgates, p.ld_dgates}};
+    for (const auto& r : rows)
+        if (r.at && ((reinterpret_cast<uintptr_t>(r.at) & 7) || (r.ld & 1))) return false;
+    return true;
+}
+
+template <bool BWD>
+int dispatch(const ScanArgs& p, int candidate, cudaStream_t s) {
     const int64_t channels = (int64_t)p.batch * p.hidden;
-    const int64_t ch = blockIdx.x * (int64_t)kSerialThreads + threadIdx.x;
-    if (ch >= channels) return;
-    const int b = (int)(ch / p.hidden), j = (int)(ch - (int64_t)b * p.hidden);
-    const int len = p.lengths ? min(max(p.lengths[b], 0), p.seq) : p.seq;
-    const int64_t step_g = (int64_t)p.batch * p.ld_gates, step_o = (int64_t)p.batch * p.ld_out;
-    const int64_t step_d = (int64_t)p.batch * p.ld_dout, step_dg = (int64_t)p.batch * p.ld_dgates;
-    const float* g = p.gates + b * p.ld_gates + j;
-    const float* o = p.out_in + b * p.ld_out + j;
-    const float* d = p.dout ? p.dout + b * p.ld_dout + j : nullptr;
-    float* dg = p.dgates + b * p.ld_dgates + j;
-    const float h_first = p.h0 ? p.h0[ch] : 0.0f;
-    const int first = p.reverse ? len - 1 : 0;  // the step that started from h0
-    float e = p.dh_n ? p.dh_n[ch] : 0.0f;
-    for (int s = 0; s < p.seq; ++s) {
-        const int t = p.reverse ? s : p.seq - 1 - s;
-        float da = 0.0f, dc = 0.0f;
-        if (t < len) {
-            float z, rest;
-            gate(g[t * step_g], z, rest);
-            const float n = candidate<TANH>(g[t * step_g + p.hidden]);
-            const float h = t == first ? h_first : o[(p.reverse ? t + 1 : t - 1) * step_o];
-            const float G = e + (d ? d[t * step_d] : 0.0f);
-            da = G * ((h - n) * (z * rest));
-            dc = G * (TANH ? rest * (1.0f - n * n) : rest);
-            e = z * G;
-        }
-        dg[t * step_dg] = da;
-        dg[t * step_dg + p.hidden] = dc;
-    }
-    if (p.dh0) p.dh0[ch] = e;
+    const bool few = p.seq > 16 && (channels + 63) / 64 * 8 <= sm_count();
+    const bool two = pairs_ok(p) && !few;
+    if (candidate == JST_SCAN_TANH) return two ? run_scan<BWD, true, 2>(p, s) : run_scan<BWD, true, 1>(p, s);
+    return two ? run_scan<BWD, false, 2>(p, s) : run_scan<BWD, false, 1>(p, s);
 }
 
-int check(const char* what, const ScanArgs& p, int candidate, bool backward) {
+int check(const ScanArgs& p, int candidate, bool backward) {
     if (p.seq < 0 || p.batch < 0 || p.hidden < 0) return set_status(JST_ERR_ARG, "scan: negative size");
     if (candidate != JST_SCAN_TANH && candidate != JST_SCAN_IDENTITY)
         return set_status(JST_ERR_ARG, "scan: unknown candidate function");
@@ -132,6 +605,10 @@ int check(const char* what, const ScanArgs& p, int candidate, bool backward) {
     if (rows == 0 || H == 0) return JST_OK;
     const int64_t most = INT64_MAX / 8 / rows;
     if (p.ld_gates < 2 * H || p.ld_out < H) return set_status(JST_ERR_ARG, "scan: pitch too small");
+    // a warp's channels may lie in 64 rows: their distance is held in 32 bits
+    const int64_t wide = 1 << 24;
+    if (p.ld_gates >= wide || p.ld_out >= wide || (backward && (p.ld_dgates >= wide || (p.dout && p.ld_dout >= wide))))
+        return set_status(JST_ERR_ARG, "scan: pitch >= 2^24");
     if (p.ld_gates > most || p.ld_out > most) return set_status(JST_ERR_ARG, "scan: size exceeds 64 bits");
     if (!p.gates) return set_status(JST_ERR_ARG, "scan: null gates");
     const int64_t span_g = ((rows - 1) * p.ld_gates + 2 * H) * 4, span_o = ((rows - 1) * p.ld_out + H) * 4;
@@ -158,7 +635,6 @@ int check(const char* what, const ScanArgs& p, int candidate, bool backward) {
     }
     if (p.dh0 && ranges_overlap(p.dh0, state, p.dgates, span_dg))
         return set_status(JST_ERR_ARG, "scan backward: dh0 overlaps dgates");
-    (void)what;
     return JST_OK;
 }
 
@@ -188,21 +664,17 @@ extern "C" int jst_scan_forward(const float* gates, int64_t ld_gates, int seq, i
     p.h0 = h0; p.lengths = lengths;
     p.out = out; p.ld_out = ld_out; p.h_n = h_n;
     p.seq = seq; p.batch = batch; p.hidden = hidden; p.reverse = reverse != 0;
-    int rc = check("scan", p, candidate, false);
+    int rc = check(p, candidate, false);
     if (rc) return rc;
     rc = require_device();
     if (rc) return rc;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    p.err = device_error_word();
     const int64_t channels = (int64_t)batch * hidden;
     if (channels == 0) return set_status(JST_OK, nullptr);
     if (seq == 0) return pass_state(h_n, h0, channels, s);
-    {
-        ProfScope prof(s, KID_SCAN);
-        const unsigned grid = (unsigned)((channels + kSerialThreads - 1) / kSerialThreads);
-        if (candidate == JST_SCAN_TANH) scan_forward_serial_kernel<true><<<grid, kSerialThreads, 0, s>>>(p);
-        else scan_forward_serial_kernel<false><<<grid, kSerialThreads, 0, s>>>(p);
-    }
-    return launched("scan launch failed");
+    rc = dispatch<false>(p, candidate, s);
+    return rc ? rc : launched("scan launch failed");
 }
 
 extern "C" int jst_scan_backward(const float* gates, int64_t ld_gates, int seq, int batch, int hidden, const float* h0,
@@ -217,19 +689,15 @@ extern "C" int jst_scan_backward(const float* gates, int64_t ld_gates, int seq, 
     p.dout = dout; p.ld_dout = ld_dout; p.dh_n = dh_n;
     p.dgates = dgates; p.ld_dgates = ld_dgates; p.dh0 = dh0;
     p.seq = seq; p.batch = batch; p.hidden = hidden; p.reverse = reverse != 0;
-    int rc = check("scan backward", p, candidate, true);
+    int rc = check(p, candidate, true);
     if (rc) return rc;
     rc = require_device();
     if (rc) return rc;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    p.err = device_error_word();
     const int64_t channels = (int64_t)batch * hidden;
     if (channels == 0) return set_status(JST_OK, nullptr);
     if (seq == 0) return pass_state(dh0, dh_n, channels, s);
-    {
-        ProfScope prof(s, KID_SCAN);
-        const unsigned grid = (unsigned)((channels + kSerialThreads - 1) / kSerialThreads);
-        if (candidate == JST_SCAN_TANH) scan_backward_serial_kernel<true><<<grid, kSerialThreads, 0, s>>>(p);
-        else scan_backward_serial_kernel<false><<<grid, kSerialThreads, 0, s>>>(p);
-    }
-    return launched("scan backward launch failed");
+    rc = dispatch<true>(p, candidate, s);
+    return rc ? rc : launched("scan backward launch failed");
 }

@@ -454,19 +454,22 @@ def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, 
     Returns {name: (value, bound)} for out, h_n and, with_grads, dgates, dh0.
 
     The bounds carry first-order rounding errors through the recurrence, u =
-    2^-24.  One exponential of -|a| (2 ulp = 4u) gives big = 1 / (1 + e) (its
-    own sum 1u, division 2 ulp = 4u, and e / (1 + e) of e's error) and small =
-    e * big (e's 4u, big's error, 1u), so the larger of z and 1 - z is off by
-    5u + 4u * small and the smaller by 14u, relative.  tanh is 2 ulp = 4u.
+    2^-24.  One exponential e of -a (a power of two to 2^-22 = 4u, and 2
+    roundings) gives z = 1 / (1 + e) (its sum 1u, the reciprocal 1 ulp = 2u, and
+    e / (1 + e) = 1 - z of e's error) and 1 - z as e z (z of e's error remains,
+    z's roundings, 1u), so the larger of z and 1 - z is off by 5u + 6u of the
+    smaller, and the smaller by 14u, relative.  tanh as (1 - t) / (1 + t) from t = exp(-2 |c|)
+    <= 0.3 (|c| >= 0.6) has 6u t / (1 - t) and 6u t / (1 + t) of t's error, two
+    sums, a reciprocal and a product: 9u; nearer to 0 it is a polynomial's 3u.
     Each step then rounds a product and a sum, and a scan that composes steps
     (products of z) rounds once more a step: 3u.  The few compositions of a
-    scan's tree add 16u once.  Below 2^-126 fp32 is a grid of 2^-149: an
-    exponential there is off by 2 of its steps whatever its size and every
-    rounding by half of one, which the factors that they meet carry on: 8
-    steps, 2^-146, a recurrence step times those factors.  m and g are the magnitudes (the same sums of
+    scan's tree add 16u once.  An exponential below 2^-126 may flush to 0, z may
+    be held at 1.5 2^-126 and products round to a grid of 2^-149, whatever their
+    size, which the factors that they meet carry on: 2^-125 a step times those.
+    m and g are the magnitudes (the same sums of
     absolute values) that these relative errors apply to.
     """
-    u, tiny = 2.0 ** -24, 2.0 ** -146
+    u, tiny = 2.0 ** -24, 2.0 ** -125
     gates = np.asarray(gates, dtype=np.float64)
     seq, batch, hidden = gates.shape[0], gates.shape[1], gates.shape[2] // 2
     length = np.full(batch, seq) if lengths is None else np.clip(np.asarray(lengths), 0, seq)
@@ -477,9 +480,9 @@ def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, 
     big, small = 1 / (1 + e), e / (1 + e)
     z, rest = np.where(a >= 0, big, small), np.where(a >= 0, small, big)
     n = np.tanh(c) if tanh else c
-    of_big = 5 + 4 * small
+    of_big = 5 + 6 * small
     cz, cr = np.where(a >= 0, of_big, 14.0), np.where(a >= 0, 14.0, of_big)
-    cn = 4.0 if tanh else 0.0
+    cn = 9.0 if tanh else 0.0
     times = range(seq - 1, -1, -1) if reverse else range(seq)
     h = np.zeros((batch, hidden)) if h0 is None else np.asarray(h0, dtype=np.float64)
     m, err = np.abs(h), np.zeros((batch, hidden))
@@ -512,7 +515,7 @@ def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, 
         dgates[t] = np.where(k, np.concatenate([G * diff * slope, G * dn], axis=1), 0.0)
         dgates_e[t] = np.where(k, np.concatenate([
             tiny * (Gm + 1) * (np.abs(diff) + 1) + Ge * np.abs(diff) * slope + Gm * slope * (diff_e + np.abs(diff) * (cz[t] + cr[t] + 3) * u),
-            tiny * (Gm + 1) + Ge * dn + Gm * (dn * (cr[t] + 3) * u + (rest[t] * 10 * u if tanh else 0.0))], axis=1), 0.0)
+            tiny * (Gm + 1) + Ge * dn + Gm * (dn * (cr[t] + 3) * u + (rest[t] * 20 * u if tanh else 0.0))], axis=1), 0.0)
         ge = np.where(k, z[t] * ge + u * (cz[t] + 4) * z[t] * Gm + tiny * (Gm + 1), ge)
         g, gm = np.where(k, z[t] * G, g), np.where(k, z[t] * Gm, gm)
     r["dgates"] = (dgates, dgates_e)

@@ -52,7 +52,8 @@ def _check(c, reverse, tanh):
 
 SIZES = [(1, 1, 1), (1, 3, 5), (2, 1, 32), (7, 2, 31), (8, 1, 33), (9, 5, 64), (31, 1, 8), (63, 3, 10), (64, 2, 96),
          (65, 1, 130), (127, 4, 3), (255, 1, 32), (256, 1, 36), (257, 2, 7), (1000, 1, 40), (1025, 1, 64), (2049, 2, 4),
-         (4100, 1, 12), (16, 64, 160)]
+         (4100, 1, 12), (16, 64, 160), (18, 2200, 64), (33, 300, 130), (40, 400, 51), (70, 80, 128), (300, 40, 64),
+         (17, 1, 2), (130, 3, 33)]
 
 
 @pytest.mark.parametrize("seq,batch,hidden", SIZES)
@@ -116,6 +117,22 @@ def test_extreme_gates():
     assert np.isposinf(out[100:, 0, 3]).all() and np.isnan(out[200:, 1, 7]).all()
     out[100:, 0, 3] = out[200:, 1, 7] = 0.0
     assert not out.any()
+
+
+def test_an_infinite_state_stays_infinite():
+    """z = 1 / 11 for thousands of steps: products of z underflow, the state does not change."""
+    import torch
+    from jstorch_b200 import rnn
+    for seq in (5, 60, 3000):
+        g = torch.zeros((seq, 2, 2 * 40), device="cuda")
+        g[..., :40] = -float(np.log(10.0))
+        h0 = torch.full((2, 40), float("inf"), device="cuda")
+        h0[1] = 1.0
+        out, h_n = rnn.gated_scan(g, h0)
+        assert bool(torch.isposinf(out[:, 0]).all()) and bool(torch.isposinf(h_n[0]).all())
+        assert bool(torch.isfinite(out[:, 1]).all())
+        _, dh0 = rnn.gated_scan_backward(torch.zeros_like(g), torch.zeros_like(out), None, torch.zeros_like(h0), dh_n=h0)
+        assert bool(torch.isposinf(dh0[0]).all()) and bool(torch.isfinite(dh0[1]).all())
 
 
 def test_pitches_and_optional_arguments():
