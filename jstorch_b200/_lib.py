@@ -194,65 +194,56 @@ def check_last() -> None:
     check(load().jst_get_last_status())
 
 
+def is_f32(x, device=None) -> bool:
+    """Whether x is a float32 CUDA tensor (on `device`, where one is given)."""
+    import torch
+
+    return isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.is_cuda and (device is None or x.device == device)
+
+
 def require_f32(x, name: str) -> None:
     """Raise unless x is a float32 CUDA tensor."""
     import torch
 
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if x.dtype != torch.float32:
+    if x.dtype is not torch.float32:
         raise TypeError(f"{name} must be float32 (got {x.dtype})")
     if not x.is_cuda:
         raise ValueError(f"{name} must live on a CUDA device")
 
 
-def stream_of(device, stream) -> int:
-    """The handle of `stream`, by default torch's current stream of `device`."""
+def empty(like, shape, stream, dtype=None):
+    """An uninitialised tensor on like's device, of its type by default, that
+    belongs to `stream`: memory that torch's allocator reuses in another
+    stream's order could still be in use there when `stream` writes it."""
     if stream is None:
-        import torch
-
-        return torch._C._cuda_getCurrentRawStream(device.index)  # a Stream object costs 2 us a call
-    if stream.device != device:
-        raise ValueError(f"stream belongs to {stream.device}, the tensors to {device}")
-    return stream.cuda_stream
-
-
-class _Here:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def on(device):
-    """A context with `device` current; nothing to do where it is already."""
+        return like.new_empty(shape, dtype=dtype) if dtype is not None else like.new_empty(shape)
     import torch
 
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def empty(shape, device, stream, dtype=None):
-    """An uninitialised tensor (float32 by default) that belongs to `stream`:
-    memory that torch's allocator reuses in another stream's order could still
-    be in use there when `stream` writes it."""
-    import torch
-
-    dtype = dtype or torch.float32
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
-def launch(device, stream, name: str, *args) -> None:
-    """Call the entry point `name` on `stream` with `device` current."""
-    handle = stream_of(device, stream)
-    with on(device):
-        check(getattr(load(), name)(*args, handle))
+def call(device, stream, function, *args) -> None:
+    """function(*args, stream handle) with `device` current, on `stream` (by
+    default torch's current stream of the device); raises on a status."""
+    import torch
+
+    index = device.index
+    if stream is None:
+        handle = torch._C._cuda_getCurrentRawStream(index)  # a Stream object costs 2 us a call
+    elif stream.device != device:
+        raise ValueError(f"stream belongs to {stream.device}, the tensors to {device}")
+    else:
+        handle = stream.cuda_stream
+    if torch.cuda.current_device() == index:
+        status = function(*args, handle)
+    else:
+        with torch.cuda.device(index):
+            status = function(*args, handle)
+    if status:
+        check(status)
 
 
 def header_functions(header: Path = HEADER) -> list[str]:

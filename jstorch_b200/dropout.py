@@ -50,7 +50,7 @@ def dropout(x, p: float, seed: int, offset: int = 0, *, step=None, out=None, str
     if step is not None and (step.dtype != torch.int64 or step.numel() != 1 or step.device != x.device):
         raise ValueError("step must be a one-element int64 tensor on x's device")
     if out is None:
-        out = _lib.empty(x.shape, x.device, stream)
+        out = _lib.empty(x, x.shape, stream)
     else:
         _lib.require_f32(out, "out")
         if out.shape != x.shape or out.device != x.device:
@@ -61,6 +61,6 @@ def dropout(x, p: float, seed: int, offset: int = 0, *, step=None, out=None, str
         rows, cols = max((rows, cols), (rows_o, cols_o))
         ldx = cols if x.is_contiguous() else ldx
         ldy = cols if out.is_contiguous() else ldy
-    _lib.launch(x.device, stream, "jst_dropout", x.data_ptr(), ldx, out.data_ptr(), ldy, rows, cols, float(p), seed,
-                offset, step.data_ptr() if step is not None else None)
+    _lib.call(x.device, stream, _lib.load().jst_dropout, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, cols, float(p), seed,
+              offset, step.data_ptr() if step is not None else None)
     return out

@@ -36,15 +36,17 @@ def _matrix(x, name: str):
 
 
 def _vector(v, name: str, n: int, device):
-    _lib.require_f32(v, name)
-    if v.shape != (n,) or v.device != device or (n > 1 and v.stride(0) != 1):
+    if not _lib.is_f32(v, device) or v.shape != (n,) or (n > 1 and v.stride(0) != 1):
+        _lib.require_f32(v, name)
         raise ValueError(f"{name} must be a contiguous float32 tensor with {n} elements on {device}")
     return v.data_ptr()
 
 
-def _output(out, M: int, N: int, device, stream):
+def _output(out, like, M: int, N: int, device, stream):
     if out is None:
-        return _lib.empty((M, N), device, stream), N
+        import torch
+
+        return _lib.empty(like, (M, N), stream, torch.float32), N
     _lib.require_f32(out, "out")
     if out.shape != (M, N) or out.device != device:
         raise ValueError(f"out must be a float32 tensor of shape {(M, N)} on {device}")
@@ -63,11 +65,16 @@ def quantize_rows(x, *, stream=None):
     _lib.require_f32(x, "x")
     rows, cols, ldx = _matrix(x, "x")
     pitch = max((cols + 15) // 16 * 16, 16)
-    held = _lib.empty((rows, pitch), x.device, stream, torch.int8)
-    scale = _lib.empty((rows,), x.device, stream)
-    _lib.launch(x.device, stream, "jst_quantize_rows_i8", x.data_ptr(), ldx, rows, cols, held.data_ptr(), pitch,
-                scale.data_ptr())
+    held = _lib.empty(x, (rows, pitch), stream, torch.int8)
+    scale = _lib.empty(x, (rows,), stream)
+    _lib.call(x.device, stream, _lib.load().jst_quantize_rows_i8, x.data_ptr(), ldx, rows, cols, held.data_ptr(), pitch,
+              scale.data_ptr())
     return held[:, :cols], scale
+
+
+def _run_desc(d, handle) -> int:
+    d.stream = handle
+    return _lib.load().jst_gemm_i8(ctypes.byref(d))
 
 
 def gemm_i8(a, w, a_scale, w_scale, out=None, *, bias=None, relu: bool = False, stream=None):
@@ -92,11 +99,9 @@ def gemm_i8(a, w, a_scale, w_scale, out=None, *, bias=None, relu: bool = False, 
     d.b_scale = _vector(w_scale, "w_scale", N, a.device)
     d.bias = _vector(bias, "bias", N, a.device) if bias is not None else None
     d.epilogue = (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0)
-    out, d.ldc = _output(out, M, N, a.device, stream)
+    out, d.ldc = _output(out, a, M, N, a.device, stream)
     d.C = out.data_ptr()
-    d.stream = _lib.stream_of(a.device, stream)
-    with _lib.on(a.device):
-        _lib.check(_lib.load().jst_gemm_i8(ctypes.byref(d)))
+    _lib.call(a.device, stream, _run_desc, d)
     return out
 
 
@@ -114,7 +119,7 @@ def linear_i8(x, w, w_scale, out=None, *, bias=None, relu: bool = False, stream=
         raise ValueError("x and w must live on one device")
     ws = _vector(w_scale, "w_scale", N, x.device)
     b = _vector(bias, "bias", N, x.device) if bias is not None else None
-    out, ldy = _output(out, M, N, x.device, stream)
-    _lib.launch(x.device, stream, "jst_linear_i8", x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, ws, N, b,
-                (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0), out.data_ptr(), ldy)
+    out, ldy = _output(out, x, M, N, x.device, stream)
+    _lib.call(x.device, stream, _lib.load().jst_linear_i8, x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, ws, N, b,
+              (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0), out.data_ptr(), ldy)
     return out
