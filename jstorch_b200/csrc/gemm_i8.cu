@@ -19,11 +19,20 @@
 //               32-column blocks: one scale per lane, one per column (through
 //               a 32-entry table in shared memory), bias, ReLU, then a TMA
 //               store of the 32 x 32 block (16-byte aligned C), or row by row.
+//
+// gemm_i8_tokens_kernel: up to 64 tokens.  The roles are exchanged (C[s, r]):
+// the 128-row side of the instruction holds channels, of which there are
+// plenty, and the other the tokens, padded to 16, 32 or 64 instead of 128.  The
+// call is a read of the weight, so it has to come from every SM: a cluster of
+// CTAs shares a tile's K range and adds its integer sums (exact in any order)
+// through distributed shared memory.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <climits>
+#include <cstdlib>
 #include <cstdint>
 #include <mutex>
 
@@ -64,7 +73,7 @@ struct Params {
     int64_t ldc;
     const float* r_scale;
     const float* s_scale;
-    const float* bias;  // one per channel: of S, or of R when swapped
+    const float* bias;  // one per channel
     int relu;
     int tma_store;
     uint32_t* err;
@@ -81,7 +90,87 @@ __device__ __forceinline__ void tile_at(int t, const Params& p, int bn, int* r0,
     *s0 = ((t % span) / gm) * bn;
 }
 
-template <class C, bool SWAP>
+// One epilogue warp's part of a tile: wait for the accumulator at `acc`, drain
+// TMEM lane quadrant q's 32-column blocks half, half + 2, ..., release() the
+// accumulator after the last read of it, and write C.  False: a wait gave up.
+template <int BN, class Release>
+__device__ __forceinline__ bool drain_tile(const Params& p, const CUtensorMap& tm_c, uint32_t acc, uint64_t* complete,
+                                           uint32_t phase, volatile uint32_t* err, int r0, int s0, int q, int half,
+                                           uint8_t* blk, float* tab, bool& stored, Release release) {
+    const int lane = threadIdx.x & 31;
+    const int row = r0 + q * 32 + lane;
+    const float rs = row < p.R ? __ldg(p.r_scale + row) : 0.0f;
+    int okw = 0;
+    if (lane == 0) okw = ptx::mbar_wait(complete, phase, err) && *err == 0;
+    if (!__shfl_sync(0xffffffffu, okw, 0)) return false;
+    ptx::tc_fence_after();
+    const int nblk = min((BN + 31) / 32, (p.S - s0 + 31) / 32);
+    const int last = nblk - 1 - ((nblk - 1 - half) & 1);
+    if (last < 0) {  // a warp without a block still releases the accumulator
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) release();
+    }
+#pragma unroll 1
+    for (int c = half; c < nblk; c += 2) {
+        const int col0 = s0 + c * 32;
+        const int col = min(col0 + lane, p.S - 1);
+        __syncwarp();  // the previous block's readers of the tables are done
+        tab[lane] = __ldg(p.s_scale + col);
+        tab[32 + lane] = p.bias ? __ldg(p.bias + col) : 0.0f;
+        uint32_t r[32];
+        ptx::tmem_ld_32x32b_x32(acc + ((uint32_t)(q * 32) << 16) + c * 32, r);
+        ptx::tmem_ld_wait();
+        if (c == last) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) release();
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const float4 sc = *reinterpret_cast<const float4*>(tab + j);
+            const float4 bi = *reinterpret_cast<const float4*>(tab + 32 + j);
+            const bool hb = p.bias != nullptr;
+            r[j + 0] = __float_as_uint(i8_finish((int)r[j + 0], rs, sc.x, hb, bi.x, p.relu));
+            r[j + 1] = __float_as_uint(i8_finish((int)r[j + 1], rs, sc.y, hb, bi.y, p.relu));
+            r[j + 2] = __float_as_uint(i8_finish((int)r[j + 2], rs, sc.z, hb, bi.z, p.relu));
+            r[j + 3] = __float_as_uint(i8_finish((int)r[j + 3], rs, sc.w, hb, bi.w, p.relu));
+        }
+        if (p.tma_store) {
+            if (r0 + q * 32 < p.R) {  // the box parts past R or S are not written
+                if (lane == 0 && stored) ptx::bulk_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<uint4*>(blk + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                        make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::tma_store_3d(&tm_c, blk, col0, r0 + q * 32, 0);
+                    ptx::bulk_commit();
+                }
+                stored = true;
+            }
+        } else {  // transpose through shared memory: one 128-byte row segment a store
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j)  // word j of row `lane` at j ^ lane: no bank conflicts either way
+                reinterpret_cast<uint32_t*>(blk)[lane * 32 + (j ^ lane)] = r[j];
+            __syncwarp();
+            if (col0 + lane < p.S)
+                for (int j = 0; j < 32; ++j)
+                    if (r0 + q * 32 + j < p.R)
+                        p.C[(int64_t)(r0 + q * 32 + j) * p.ldc + col0 + lane] =
+                            __uint_as_float(reinterpret_cast<uint32_t*>(blk)[j * 32 + (lane ^ j)]);
+            __syncwarp();
+        }
+    }
+    return true;
+}
+
+template <class C>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_i8_tc_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_s,
                       const __grid_constant__ CUtensorMap tm_c, const Params p) {
@@ -185,83 +274,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int buf = i & 1;
             int r0, s0;
             tile_at(t, p, BN, &r0, &s0);
-            const int row = r0 + q * 32 + lane;
-            const float rs = row < p.R ? __ldg(p.r_scale + row) : 0.0f;
-            const float rb = SWAP && p.bias && row < p.R ? __ldg(p.bias + row) : 0.0f;
-            int okw = 0;
-            if (lane == 0) okw = ptx::mbar_wait(&accf_bar[buf], (i >> 1) & 1, err) && *err == 0;
-            if (!__shfl_sync(0xffffffffu, okw, 0)) break;
-            ptx::tc_fence_after();
-            const int nblk = min((BN + 31) / 32, (p.S - s0 + 31) / 32);
-            const int last = nblk - 1 - ((nblk - 1 - half) & 1);
-            if (last < 0) {  // a warp without a block still releases the accumulator
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&acce_bar[buf]);
-            }
-#pragma unroll 1
-            for (int c = half; c < nblk; c += 2) {
-                const int col0 = s0 + c * 32;
-                const int col = min(col0 + lane, p.S - 1);
-                __syncwarp();  // the previous block's readers of the tables are done
-                tab[lane] = __ldg(p.s_scale + col);
-                if (!SWAP) tab[32 + lane] = p.bias ? __ldg(p.bias + col) : 0.0f;
-                uint32_t r[32];
-                ptx::tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + buf * C::ACC_COLS + c * 32, r);
-                ptx::tmem_ld_wait();
-                if (c == last) {
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&acce_bar[buf]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 sc = *reinterpret_cast<const float4*>(tab + j);
-                    const float4 bi = SWAP ? make_float4(rb, rb, rb, rb) : *reinterpret_cast<const float4*>(tab + 32 + j);
-                    const bool hb = p.bias != nullptr;
-                    r[j + 0] = __float_as_uint(i8_finish((int)r[j + 0], rs, sc.x, hb, bi.x, p.relu));
-                    r[j + 1] = __float_as_uint(i8_finish((int)r[j + 1], rs, sc.y, hb, bi.y, p.relu));
-                    r[j + 2] = __float_as_uint(i8_finish((int)r[j + 2], rs, sc.z, hb, bi.z, p.relu));
-                    r[j + 3] = __float_as_uint(i8_finish((int)r[j + 3], rs, sc.w, hb, bi.w, p.relu));
-                }
-                if (SWAP) {  // lanes are adjacent columns of C
-                    if (row < p.R) {
-                        float* dst = p.C + (int64_t)col0 * p.ldc + row;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col0 + j < p.S) dst[(int64_t)j * p.ldc] = __uint_as_float(r[j]);
-                    }
-                } else if (p.tma_store) {
-                    if (r0 + q * 32 < p.R) {  // the box parts past R or S are not written
-                        if (lane == 0 && stored) ptx::bulk_wait_read<0>();
-                        __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint4*>(blk + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-                        ptx::fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            ptx::tma_store_3d(&tm_c, blk, col0, r0 + q * 32, 0);
-                            ptx::bulk_commit();
-                        }
-                        stored = true;
-                    }
-                } else {  // transpose through shared memory: one 128-byte row segment a store
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)  // word j of row `lane` at j ^ lane: no bank conflicts either way
-                        reinterpret_cast<uint32_t*>(blk)[lane * 32 + (j ^ lane)] = r[j];
-                    __syncwarp();
-                    if (col0 + lane < p.S)
-                        for (int j = 0; j < 32; ++j)
-                            if (r0 + q * 32 + j < p.R)
-                                p.C[(int64_t)(r0 + q * 32 + j) * p.ldc + col0 + lane] =
-                                    __uint_as_float(reinterpret_cast<uint32_t*>(blk)[j * 32 + (lane ^ j)]);
-                    __syncwarp();
-                }
-            }
+            if (!drain_tile<BN>(p, tm_c, tmem_base + buf * C::ACC_COLS, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
+                                blk, tab, stored, [&] { ptx::mbar_arrive(&acce_bar[buf]); }))
+                break;
         }
         if (lane == 0 && stored) ptx::bulk_wait_all();  // C is written before the CTA exits
     }
@@ -272,6 +287,346 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         ptx::tc_fence_after();
         ptx::tmem_dealloc<C::TMEM_COLS>(tmem_base);
+    }
+    if (threadIdx.x == 0 && *err != 0) atomicOr(p.err, *err);
+}
+
+// ------------------------------------------------------------ pairs of SMs
+// The same walk with 256 x 256 tiles on two CTAs of a cluster (cta_group::2):
+// each stages its 128 rows of R and of S, each half of S serves both, and one
+// thread of the first issues the instructions for the two.  A CTA alone reads
+// and writes 192 bytes of shared memory for what takes the pair 128 a CTA, and
+// shared memory is what bounds gemm_i8_tc_kernel (128 bytes a cycle).
+// Barriers of the first CTA count both CTAs' loads and drained accumulators;
+// commits arrive at both.
+struct PairCfg {
+    static constexpr int STAGES = 6;
+    static constexpr int BN = 256;
+    static constexpr uint32_t HALF_BYTES = BM * BK;  // 128 rows of R, 128 rows of S
+    static constexpr uint32_t STAGE_BYTES = 2 * HALF_BYTES;
+    static constexpr uint32_t STG_OFF = STAGES * STAGE_BYTES;
+    static constexpr uint32_t TAB_OFF = STG_OFF + 8 * 4096;
+    static constexpr uint32_t BAR_OFF = TAB_OFF + 8 * 256;
+    static constexpr uint32_t SMEM_BYTES = BAR_OFF + 256 + 768;
+    static_assert(SMEM_BYTES <= 227 * 1024 && (2 * STAGES + 5) * 8 + 8 <= 256, "shared memory per CTA");
+};
+
+__device__ __forceinline__ void pair_tile_at(int t, const Params& p, int* r0, int* s0) {
+    constexpr int GROUP = 8;  // bands of 8 x 256 rows
+    const int span = GROUP * p.tiles_s;
+    const int g = t / span, first = g * GROUP;
+    const int gm = min(p.tiles_r - first, GROUP);
+    *r0 = (first + (t % span) % gm) * 2 * BM;
+    *s0 = ((t % span) / gm) * PairCfg::BN;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_s,
+                        const __grid_constant__ CUtensorMap tm_c, const Params p) {
+    using C = PairCfg;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ __align__(256) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // of the first CTA: both halves have landed
+    uint64_t* empty_bar = full_bar + STAGES;
+    uint64_t* accf_bar = empty_bar + STAGES;  // [2]
+    uint64_t* acce_bar = accf_bar + 2;        // [2] of the first CTA: both CTAs have drained it
+    uint64_t* done_bar = acce_bar + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+    volatile uint32_t* err = tmem_slot + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x & 1);
+    const int pairs = (int)(gridDim.x >> 1), pair = (int)(blockIdx.x >> 1);
+    const int total = p.tiles_r * p.tiles_s;
+    const int num_kb = (p.K + BK - 1) / BK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            ptx::mbar_init(&accf_bar[b], 1);
+            ptx::mbar_init(&acce_bar[b], 16);  // one arrival per epilogue warp of either CTA
+        }
+        ptx::mbar_init(done_bar, 1);
+        *err = 0;
+        ptx::fence_barrier_init();
+        ptx::tma_prefetch_desc(&tm_r);
+        ptx::tma_prefetch_desc(&tm_s);
+        if (p.tma_store) ptx::tma_prefetch_desc(&tm_c);
+    }
+    if (warp == 1) ptx::tmem_alloc_pair<512>(tmem_slot);
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_arrive();  // the other CTA's barriers and TMEM are ready too
+    ptx::cluster_wait();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t g = 0;
+            bool ok = true;
+            for (int t = pair; t < total && ok; t += pairs) {
+                int r0, s0;
+                pair_tile_at(t, p, &r0, &s0);
+                for (int kb = 0; kb < num_kb; ++kb, ++g) {
+                    const int s = g % STAGES;
+                    if (!ptx::mbar_wait(&empty_bar[s], ((g / STAGES) & 1) ^ 1, err)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + s * C::STAGE_BYTES;
+                    const uint32_t bar = ptx::cluster_addr(ptx::smem_u32(&full_bar[s]), 0);
+                    if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+                    ptx::tma_load_3d_pair(st, &tm_r, bar, kb * BK, r0 + rank * BM, 0);
+                    ptx::tma_load_3d_pair(st + C::HALF_BYTES, &tm_s, bar, kb * BK, s0 + rank * BM, 0);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = ptx::idesc_i8(2 * BM, C::BN);
+            uint32_t g = 0;
+            bool ok = true;
+            int i = 0;
+            for (int t = pair; t < total && ok; t += pairs, ++i) {
+                const int buf = i & 1;
+                if (!ptx::mbar_wait<true>(&acce_bar[buf], ((i >> 1) & 1) ^ 1, err)) break;
+                ptx::tc_fence_after();
+                const uint32_t d = tmem_base + buf * C::BN;
+                for (int kb = 0; kb < num_kb; ++kb, ++g) {
+                    const int s = g % STAGES;
+                    if (!ptx::mbar_wait(&full_bar[s], (g / STAGES) & 1, err)) {
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after();
+                    const uint32_t st = ptx::smem_u32(smem + s * C::STAGE_BYTES);
+#pragma unroll
+                    for (int kk = 0; kk < BK / 32; ++kk)
+                        ptx::mma_i8_pair(d, ptx::smem_desc_kmajor(st + kk * 32, 128),
+                                         ptx::smem_desc_kmajor(st + C::HALF_BYTES + kk * 32, 128), idesc, (kb | kk) != 0);
+                    ptx::mma_commit_pair(&empty_bar[s]);
+                }
+                if (ok) ptx::mma_commit_pair(&accf_bar[buf]);
+            }
+            ptx::mma_commit_pair(done_bar);
+            ptx::mbar_wait(done_bar, 0, err);  // every MMA completes before the TMEM is released
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;
+        const int half = (warp - 2) >> 2;
+        uint8_t* blk = smem + C::STG_OFF + (warp - 2) * 4096;
+        float* tab = reinterpret_cast<float*>(smem + C::TAB_OFF + (warp - 2) * 256);
+        bool stored = false;
+        int i = 0;
+        for (int t = pair; t < total; t += pairs, ++i) {
+            const int buf = i & 1;
+            int r0, s0;
+            pair_tile_at(t, p, &r0, &s0);
+            r0 += rank * BM;
+            const uint32_t drained = ptx::cluster_addr(ptx::smem_u32(&acce_bar[buf]), 0);
+            if (!drain_tile<C::BN>(p, tm_c, tmem_base + buf * C::BN, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
+                                   blk, tab, stored, [&] { ptx::mbar_arrive_cluster(drained); }))
+                break;
+        }
+        if (lane == 0 && stored) ptx::bulk_wait_all();
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {  // the last commit's arrival here, before this CTA may leave
+        if (lane == 0 && rank == 1) ptx::mbar_wait(done_bar, 0, err);
+        __syncwarp();
+    }
+    ptx::cluster_arrive();  // neither CTA leaves, or frees its TMEM, while the other's work may touch it
+    ptx::cluster_wait();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair<512>(tmem_base);
+    }
+    if (threadIdx.x == 0 && *err != 0) atomicOr(p.err, *err);
+}
+
+// ------------------------------------------------------------ few tokens
+template <int T_, int STAGES_>
+struct TokCfg {
+    static constexpr int T = T_;  // tokens, padded
+    static constexpr int STAGES = STAGES_;
+    static constexpr uint32_t TMEM_COLS = T_ < 32 ? 32 : T_;
+    static constexpr uint32_t R_BYTES = BM * BK;
+    static constexpr uint32_t S_BYTES = T_ * BK;
+    static constexpr uint32_t STAGE_BYTES = R_BYTES + S_BYTES;
+    static constexpr uint32_t EX_OFF = STAGES_ * STAGE_BYTES;  // int32 [cluster][128][tokens of this CTA]
+    static constexpr uint32_t SCALE_OFF = EX_OFF + T_ * BM * 4;
+    static constexpr uint32_t BAR_OFF = SCALE_OFF + 256;
+    static constexpr uint32_t SMEM_BYTES = BAR_OFF + 256 + 768 /*from 256- to 1024-byte alignment*/;
+    static_assert(SMEM_BYTES <= 227 * 1024 && S_BYTES % 1024 == 0 && (2 * STAGES_ + 1) * 8 + 8 <= 256, "shared memory");
+};
+constexpr int TOK_THREADS = 192;
+
+struct TokParams {
+    int channels, tokens, K;
+    int cluster_log2, kb_per_rank;  // CTAs that share a tile (at most T / 4), k-slabs of each
+    float* C;
+    int64_t ldc;
+    const float* channel_scale;
+    const float* token_scale;
+    const float* bias;
+    int relu;
+    uint32_t* err;
+};
+
+//   warp 0      TMA producer (and, before it may read what the launch before
+//               this one wrote, prefetches of its weight slabs into L2)
+//   warp 1      TMEM allocation, MMA issue
+//   warps 2-5   exchange and epilogue, a lane a channel
+template <class C>
+__global__ void __launch_bounds__(TOK_THREADS)
+    gemm_i8_tokens_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                          const TokParams p) {
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ __align__(256) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    int* exchange = reinterpret_cast<int*>(smem + C::EX_OFF);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+    uint64_t* empty_bar = full_bar + STAGES;
+    uint64_t* accum_bar = empty_bar + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum_bar + 1);
+    volatile uint32_t* err = tmem_slot + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* token_scale = reinterpret_cast<float*>(smem + C::SCALE_OFF);
+    const int cluster = 1 << p.cluster_log2;
+    const int rank = (int)(blockIdx.x & (cluster - 1));
+    const int n0 = (int)(blockIdx.x >> p.cluster_log2) * BM;
+    const int kb0 = rank * p.kb_per_rank;
+    const int num_kb = max(0, min((p.K + BK - 1) / BK - kb0, p.kb_per_rank));
+    const int own = C::T >> p.cluster_log2, own0 = rank * own;  // the tokens whose sums meet in this CTA: a multiple of 4
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        ptx::mbar_init(accum_bar, 1);
+        *err = 0;
+        ptx::fence_barrier_init();
+        ptx::tma_prefetch_desc(&tm_w);
+        ptx::tma_prefetch_desc(&tm_x);
+        for (int kb = 0; kb < num_kb; ++kb) ptx::tma_prefetch_3d(&tm_w, (kb0 + kb) * BK, n0, 0);
+    }
+    if (warp == 1) ptx::tmem_alloc<C::TMEM_COLS>(tmem_slot);
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    if (threadIdx.x < own) token_scale[threadIdx.x] = own0 + threadIdx.x < p.tokens ? __ldg(p.token_scale + own0 + threadIdx.x) : 0.0f;
+    if (cluster > 1) {  // nobody writes another's shared memory before that one runs
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int kb = 0; kb < num_kb; ++kb) {
+                const int s = kb % STAGES;
+                if (!ptx::mbar_wait(&empty_bar[s], ((kb / STAGES) & 1) ^ 1, err)) break;
+                uint8_t* st = smem + s * C::STAGE_BYTES;
+                ptx::mbar_arrive_expect_tx(&full_bar[s], C::STAGE_BYTES);
+                ptx::tma_load_3d(st, &tm_w, &full_bar[s], (kb0 + kb) * BK, n0, 0);
+                ptx::tma_load_3d(st + C::R_BYTES, &tm_x, &full_bar[s], (kb0 + kb) * BK, 0, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = ptx::idesc_i8(BM, C::T);
+            for (int kb = 0; kb < num_kb; ++kb) {
+                const int s = kb % STAGES;
+                if (!ptx::mbar_wait(&full_bar[s], (kb / STAGES) & 1, err)) break;
+                ptx::tc_fence_after();
+                const uint32_t st = ptx::smem_u32(smem + s * C::STAGE_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < BK / 32; ++kk)
+                    ptx::mma_i8(tmem_base, ptx::smem_desc_kmajor(st + kk * 32, 128),
+                                ptx::smem_desc_kmajor(st + C::R_BYTES + kk * 32, 128), idesc, (kb | kk) != 0);
+                ptx::mma_commit(&empty_bar[s]);
+            }
+            ptx::mma_commit(accum_bar);  // always signalled, also on the error path
+            ptx::mbar_wait(accum_bar, 0, err);
+        }
+        __syncwarp();
+    } else {
+        int okw = 0;
+        if (lane == 0) okw = ptx::mbar_wait(accum_bar, 0, err) && *err == 0;
+        const bool ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+        ptx::tc_fence_after();
+        const int q = warp & 3;  // TMEM lane quadrant this warp may access
+        const int row = q * 32 + lane;
+        if (ok) {
+            // this lane's channel: its partial sums of the tokens, four at a
+            // time, to the CTA that owns those
+#pragma unroll 1
+            for (int c = 0; c < C::T && c < p.tokens; c += 16) {
+                uint32_t r[16];
+                if (num_kb > 0) {
+                    ptx::tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(q * 32) << 16) + c, r);
+                    ptx::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) r[j] = 0;
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const int owner = (c + j) / own, at = (rank * BM + row) * own + (c + j) % own;  // own: a power of two
+                    if (cluster > 1)
+                        ptx::cluster_store_v4(ptx::cluster_addr(ptx::smem_u32(exchange + at), owner), r[j], r[j + 1],
+                                              r[j + 2], r[j + 3]);
+                    else
+                        *reinterpret_cast<uint4*>(exchange + at) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+                }
+            }
+        }
+    }
+    ptx::tc_fence_before();
+    if (cluster > 1) {  // every sum has arrived; nobody leaves before
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<C::TMEM_COLS>(tmem_base);
+    } else if (warp >= 2 && *err == 0) {
+        const int row = (warp & 3) * 32 + lane, n = n0 + row;
+        if (n < p.channels) {
+            const float cs = __ldg(p.channel_scale + n), bias = p.bias ? __ldg(p.bias + n) : 0.0f;
+            float* out = p.C + (int64_t)own0 * p.ldc + n;
+            for (int i = 0; i < own && own0 + i < p.tokens; i += 4) {
+                int4 sum = make_int4(0, 0, 0, 0);
+                for (int o = 0; o < cluster; ++o) {
+                    const int4 v = *reinterpret_cast<const int4*>(exchange + (o * BM + row) * own + i);
+                    sum = make_int4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+                }
+                const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (own0 + i + j < p.tokens)
+                        out[(i + j) * p.ldc] = i8_finish(v[j], token_scale[i + j], cs, p.bias != nullptr, bias, p.relu);
+            }
+        }
     }
     if (threadIdx.x == 0 && *err != 0) atomicOr(p.err, *err);
 }
@@ -320,7 +675,7 @@ static bool make_map(CUtensorMap* m, const void* base, CUtensorMapDataType type,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class Cf, bool SWAP>
+template <class Cf>
 static int launch(const CUtensorMap& r, const CUtensorMap& s, const CUtensorMap& c, const Params& p, cudaStream_t st) {
     static bool attr_set[64] = {};
     static std::mutex mu;
@@ -329,7 +684,7 @@ static int launch(const CUtensorMap& r, const CUtensorMap& s, const CUtensorMap&
     {
         std::lock_guard<std::mutex> lk(mu);
         if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-            if (cudaFuncSetAttribute(gemm_i8_tc_kernel<Cf, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            if (cudaFuncSetAttribute(gemm_i8_tc_kernel<Cf>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      Cf::SMEM_BYTES) != cudaSuccess)
                 return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(gemm_i8_tc_kernel) failed");
             attr_set[dev] = true;
@@ -337,7 +692,7 @@ static int launch(const CUtensorMap& r, const CUtensorMap& s, const CUtensorMap&
     }
     const unsigned grid = (unsigned)std::min<int64_t>((int64_t)p.tiles_r * p.tiles_s, sm_count());
     ProfScope prof(st, KID_GEMM_I8);
-    if (launch_dependent(gemm_i8_tc_kernel<Cf, SWAP>, dim3(grid), dim3(THREADS), Cf::SMEM_BYTES, st, r, s, c, p) !=
+    if (launch_dependent(gemm_i8_tc_kernel<Cf>, dim3(grid), dim3(THREADS), Cf::SMEM_BYTES, st, r, s, c, p) !=
         cudaSuccess)
         return set_status(JST_ERR_CUDA, "gemm_i8_tc_kernel launch failed");
     return JST_OK;
@@ -360,46 +715,118 @@ static int realign(const int8_t** x, int64_t* ld, int rows, int cols, int8_t* to
     return JST_OK;
 }
 
-static int run_aligned(const I8Args& a, cudaStream_t s) {
-    Params p{};
-    p.K = a.K;
+static int launch_pair(const CUtensorMap& r, const CUtensorMap& s, const CUtensorMap& c, const Params& p, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    static std::mutex mu;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+            if (cudaFuncSetAttribute(gemm_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     PairCfg::SMEM_BYTES) != cudaSuccess)
+                return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(gemm_i8_pair_kernel) failed");
+            attr_set[dev] = true;
+        }
+    }
+    const unsigned grid = 2 * (unsigned)std::min<int64_t>((int64_t)p.tiles_r * p.tiles_s, sm_count() / 2);
+    ProfScope prof(st, KID_GEMM_I8);
+    if (launch_dependent(gemm_i8_pair_kernel, dim3(grid), dim3(THREADS), PairCfg::SMEM_BYTES, st, r, s, c, p) != cudaSuccess)
+        return set_status(JST_ERR_CUDA, "gemm_i8_pair_kernel launch failed");
+    return JST_OK;
+}
+
+template <class Cf>
+static int launch_tokens(const CUtensorMap& w, const CUtensorMap& x, const TokParams& p, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    static std::mutex mu;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+            if (cudaFuncSetAttribute(gemm_i8_tokens_kernel<Cf>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     Cf::SMEM_BYTES) != cudaSuccess)
+                return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(gemm_i8_tokens_kernel) failed");
+            attr_set[dev] = true;
+        }
+    }
+    const int cluster = 1 << p.cluster_log2;
+    const unsigned grid = (unsigned)((p.channels + BM - 1) / BM * cluster);
+    ProfScope prof(st, KID_GEMM_I8);
+    if (launch_dependent_cluster(gemm_i8_tokens_kernel<Cf>, dim3(grid), dim3(TOK_THREADS), cluster, Cf::SMEM_BYTES, st,
+                                 w, x, p) != cudaSuccess)
+        return set_status(JST_ERR_CUDA, "gemm_i8_tokens_kernel launch failed");
+    return JST_OK;
+}
+
+// The pitch of a single row is never used, but a map wants a multiple of 16 bytes.
+static bool make_operand_map(CUtensorMap* m, const int8_t* x, int rows, int K, int64_t ld, int box_rows) {
+    return make_map(m, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, rows, rows == 1 ? ((int64_t)K + 15) / 16 * 16 : ld, box_rows);
+}
+
+static int run_tokens(const I8Args& a, cudaStream_t s) {
+    const int T = a.M <= 16 ? 16 : a.M <= 32 ? 32 : 64;
+    CUtensorMap w, x;
+    if (!make_operand_map(&w, a.B, a.N, a.K, a.ldb, BM) || !make_operand_map(&x, a.A, a.M, a.K, a.lda, T))
+        return set_status(JST_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    TokParams p{};
+    p.channels = a.N; p.tokens = a.M; p.K = a.K;
     p.C = a.C; p.ldc = a.ldc;
+    p.channel_scale = a.b_scale; p.token_scale = a.a_scale;
     p.bias = a.bias; p.relu = a.relu;
     p.err = device_error_word();
-    const bool swap = a.M <= 64;
-    int bn;
-    if (swap) {
-        bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : 64;
-    } else {
-        // the widest tile that still gives every SM one
-        const int64_t rows = (a.M + BM - 1) / BM, sms = sm_count();
-        bn = rows * ((a.N + 255) / 256) >= sms ? 256 : rows * ((a.N + 127) / 128) >= sms ? 128 : 64;
+    // CTAs that share a tile: as many as the SMs take (two CTAs of up to 32
+    // tokens fit one), with a k-slab and four tokens at least each (16 tokens,
+    // 4096 x 4096: 15.6 us alone, 10.4 with two, 7.9 with four; 16, 2048 x 512:
+    // 5.3, 4.8, 4.2; 64, 8192 x 8192: 34.1, 21.6, and 28.4 with four, which no
+    // longer run at the same time)
+    const int tiles = (a.N + BM - 1) / BM, slabs = (a.K + BK - 1) / BK, room = sm_count() * (T <= 32 ? 2 : 1);
+    int lg = 0;
+    while (lg < 3 && (8 << lg) <= T && (tiles << (lg + 1)) <= room && (2 << lg) <= slabs) ++lg;
+    p.cluster_log2 = lg;
+    p.kb_per_rank = (slabs + (1 << lg) - 1) >> lg;
+    if (T == 16) return launch_tokens<TokCfg<16, 5>>(w, x, p, s);
+    if (T == 32) return launch_tokens<TokCfg<32, 4>>(w, x, p, s);
+    return launch_tokens<TokCfg<64, 7>>(w, x, p, s);
+}
+
+static int run_aligned(const I8Args& a, cudaStream_t s) {
+    if (a.M <= 64) return run_tokens(a, s);
+    // Waves of tiles times what a tile costs a k-slab: the 128 token rows that
+    // it stages whatever its width, and its own BN rows.
+    const int64_t rows = (a.M + BM - 1) / BM, sms = sm_count();
+    int bn = 256;
+    int64_t best = INT64_MAX;
+    for (int n : {256, 128, 64}) {
+        const int64_t waves = (rows * ((a.N + n - 1) / n) + sms - 1) / sms, cost = waves * (n + 64);
+        if (cost < best) {
+            best = cost;
+            bn = n;
+        }
     }
-    const int8_t *r = swap ? a.B : a.A, *q = swap ? a.A : a.B;
-    const int64_t ldr = swap ? a.ldb : a.lda, lds = swap ? a.lda : a.ldb;
-    p.R = swap ? a.N : a.M;
-    p.S = swap ? a.M : a.N;
-    p.r_scale = swap ? a.b_scale : a.a_scale;
-    p.s_scale = swap ? a.a_scale : a.b_scale;
-    p.tiles_r = (p.R + BM - 1) / BM;
+    const char* e = getenv("JST_PAIR");
+    const bool pair = e && atoi(e);
+    if (pair) bn = 256;
+    Params p{};
+    p.R = a.M; p.S = a.N; p.K = a.K;
+    p.C = a.C; p.ldc = a.ldc;
+    p.r_scale = a.a_scale; p.s_scale = a.b_scale;
+    p.bias = a.bias; p.relu = a.relu;
+    p.err = device_error_word();
+    p.tiles_r = pair ? (p.R + 2 * BM - 1) / (2 * BM) : (p.R + BM - 1) / BM;
     p.tiles_s = (p.S + bn - 1) / bn;
     if ((int64_t)p.tiles_r * p.tiles_s > 0x7fffffff) return set_status(JST_ERR_ARG, "gemm_i8: too many tiles");
-    const int64_t one = ((int64_t)a.K + 15) / 16 * 16;  // the pitch of a single row is never used
     CUtensorMap mr, ms, mc;
-    if (!make_map(&mr, r, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, p.R, p.R == 1 ? one : ldr, BM) ||
-        !make_map(&ms, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, p.S, p.S == 1 ? one : lds, bn))
+    if (!make_operand_map(&mr, a.A, a.M, a.K, a.lda, BM) || !make_operand_map(&ms, a.B, a.N, a.K, a.ldb, pair ? BM : bn))
         return set_status(JST_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     mc = mr;  // not read unless tma_store
-    p.tma_store = !swap && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 && (a.ldc & 3) == 0 &&
+    p.tma_store = (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 && (a.ldc & 3) == 0 &&
                   make_map(&mc, a.C, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, a.N, a.M, a.ldc, 32);
-    if (swap) {
-        if (bn == 16) return launch<Cfg<16, 8>, true>(mr, ms, mc, p, s);
-        if (bn == 32) return launch<Cfg<32, 8>, true>(mr, ms, mc, p, s);
-        return launch<Cfg<64, 6>, true>(mr, ms, mc, p, s);
-    }
-    if (bn == 256) return launch<Cfg<256, 4>, false>(mr, ms, mc, p, s);
-    if (bn == 128) return launch<Cfg<128, 5>, false>(mr, ms, mc, p, s);
-    return launch<Cfg<64, 6>, false>(mr, ms, mc, p, s);
+    if (pair) return launch_pair(mr, ms, mc, p, s);
+    if (bn == 256) return launch<Cfg<256, 4>>(mr, ms, mc, p, s);
+    if (bn == 128) return launch<Cfg<128, 5>>(mr, ms, mc, p, s);
+    return launch<Cfg<64, 6>>(mr, ms, mc, p, s);
 }
 
 }  // namespace i8

@@ -39,44 +39,90 @@ __device__ __forceinline__ float row_inverse(float s) { return s > 0.0f ? __fdiv
 
 __device__ __forceinline__ int quantize_in(float x, float s, float inv) { return inv > 0.0f ? quantize(x, s, inv) : 0; }
 
-constexpr int kQuantThreads = 256;
-
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const float* __restrict__ x, int64_t ldx,
-                                                                      int cols, int8_t* __restrict__ q, int64_t ldq,
-                                                                      float* __restrict__ scale) {
-    __shared__ uint32_t part[kQuantThreads / 32];
+// One block a row.  NV > 0: the row's values stay in registers, NV groups of
+// four a thread, between the peak and the quantisation, so x is read once;
+// NV == 0 (rows of more than 32768 values) reads it twice.  Bound by memory: 5
+// bytes a value.  VEC: x and q rows allow 16- and 4-byte accesses.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(const float* __restrict__ x, int64_t ldx, int cols, int8_t* __restrict__ q,
+                                     int64_t ldq, float* __restrict__ scale) {
+    __shared__ uint32_t part[32];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
     const float* row = x + (int64_t)blockIdx.x * ldx;
     int8_t* out = q + (int64_t)blockIdx.x * ldq;
+    const int n = blockDim.x;
+    auto fetch = [&](int k) {
+        if (VEC && k + 4 <= cols) return __ldcs(reinterpret_cast<const float4*>(row + k));
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < cols) v.x = row[k];
+        if (k + 1 < cols) v.y = row[k + 1];
+        if (k + 2 < cols) v.z = row[k + 2];
+        if (k + 3 < cols) v.w = row[k + 3];
+        return v;
+    };
+    auto put = [&](int k, float4 v, float s, float inv) {
+        const int a = quantize_in(v.x, s, inv), b = quantize_in(v.y, s, inv), c = quantize_in(v.z, s, inv),
+                  d = quantize_in(v.w, s, inv);
+        if (VEC && k + 4 <= cols) {
+            *reinterpret_cast<char4*>(out + k) = make_char4((signed char)a, (signed char)b, (signed char)c, (signed char)d);
+            return;
+        }
+        if (k < cols) out[k] = (int8_t)a;
+        if (k + 1 < cols) out[k + 1] = (int8_t)b;
+        if (k + 2 < cols) out[k + 2] = (int8_t)c;
+        if (k + 3 < cols) out[k + 3] = (int8_t)d;
+    };
+    float4 v[NV ? NV : 1];
     uint32_t m = 0;
-    for (int k = threadIdx.x; k < cols; k += kQuantThreads) m = max(m, abs_bits(row[k]));
+    auto peak = [&](const float4& f) {
+        m = max(max(max(m, abs_bits(f.x)), max(abs_bits(f.y), abs_bits(f.z))), abs_bits(f.w));
+    };
+    if (NV) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = fetch(4 * (threadIdx.x + i * n));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) peak(v[i]);
+    } else {
+        for (int k = 4 * threadIdx.x; k < cols; k += 4 * n) peak(fetch(k));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
-    for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, part[w]);
+    m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < n / 32 ? part[threadIdx.x & 31] : 0u);
     const float s = row_scale(m), inv = row_inverse(s);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
-    for (int k = threadIdx.x; k < cols; k += kQuantThreads) out[k] = (int8_t)quantize_in(row[k], s, inv);
+    if (NV) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) put(4 * (threadIdx.x + i * n), v[i], s, inv);
+    } else {
+        for (int k = 4 * threadIdx.x; k < cols; k += 4 * n) put(k, fetch(k), s, inv);
+    }
 }
 
-// ------------------------------------------------------------ a few tokens
-// C[m, n] for MT <= 8 tokens.  A warp takes kChannels rows of the weight and
-// walks along K, 16 bytes a lane and row: one 16-byte piece of a token from
-// shared memory meets kChannels pieces of the weight, 4 dp4a each.  The
-// lanes' sums meet in one integer reduction, exact in any order.
-// Bound by the weight's bytes; each is read once.
-// The tokens are held in shared memory kSegment values of K at a time.  FUSED:
-// they come as fp32 rows and every block quantises them itself.
+// ------------------------------------------------------------ one token
+// A warp takes CH rows of the weight and walks along K, 16 bytes a lane and
+// row: one 16-byte piece of the token from shared memory meets CH pieces
+// of the weight, 4 dp4a each.  The lanes' sums meet in one integer reduction,
+// exact in any order.
+// Bound by the weight's bytes; each is read once, and asked of DRAM (a prefetch
+// into L2) before the block turns to the token or waits for the launch before.
+// The token is held in shared memory kSegment values of K at a time.  NV > 0
+// (K <= 1024 NV): it comes as fp32 values and every block quantises it itself,
+// NV groups of four a thread.
 // ALIGN: 16 when the weight's rows are 16-byte aligned.  Otherwise 1: a lane
 // reads the aligned 4-byte words that hold its 16 bytes and shifts; a word that
 // holds a byte of the row does not leave the memory block that the row is in.
-constexpr int kFewThreads = 256;
-constexpr int kChannels = 4;
+// Two rows a warp and four pieces of each in flight: 8192 x 8192 in 16.5 us
+// (4.1 TB/s; a row maximum of as many bytes takes 14.6), with one row 16.8 and
+// with four 23.7; quantising the token here adds 1.2 us, a launch of its own 4.
+constexpr int kOneThreads = 256;
+constexpr int CH = 2;
 constexpr int kSegment = 8192;
 
-struct FewArgs {
-    I8Args p;        // FUSED: A and a_scale are unused
-    const float* x;  // FUSED: [M][K] fp32
-    int64_t ldx;
+struct OneArgs {
+    I8Args p;        // NV > 0: A and a_scale are unused
+    const float* x;  // NV > 0: [K] fp32
 };
 
 template <int ALIGN>
@@ -97,106 +143,118 @@ __device__ __forceinline__ int dot16(int4 a, int4 b, int c) {
     return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, c))));
 }
 
-template <int MT, int ALIGN, bool FUSED>
-__global__ void __launch_bounds__(kFewThreads) gemm_i8_few_kernel(const FewArgs f) {
-    extern __shared__ __align__(16) int8_t tokens[];  // [MT][seg], seg a multiple of 16
-    __shared__ uint32_t part[MT][kFewThreads / 32];
-    __shared__ float scales[MT], inverses[MT];
-    ptx::griddep_wait();
-    ptx::griddep_launch_dependents();
+template <int ALIGN, int NV>
+__global__ void __launch_bounds__(kOneThreads) gemm_i8_one_kernel(const OneArgs f) {
+    __shared__ __align__(16) int8_t token[kSegment];
+    __shared__ uint32_t part[kOneThreads / 32];
     const I8Args& p = f.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n0 = (blockIdx.x * (kFewThreads / 32) + warp) * kChannels;
-    if (FUSED) {
-        for (int m = 0; m < MT; ++m) {
-            uint32_t peak = 0;
-            if (m < p.M)
-                for (int k = threadIdx.x; k < p.K; k += kFewThreads) peak = max(peak, abs_bits(__ldg(f.x + m * f.ldx + k)));
-            peak = __reduce_max_sync(0xffffffffu, peak);
-            if (lane == 0) part[m][warp] = peak;
-        }
-        __syncthreads();
-        if (threadIdx.x < MT) {
-            uint32_t peak = 0;
-            for (int w = 0; w < kFewThreads / 32; ++w) peak = max(peak, part[threadIdx.x][w]);
-            scales[threadIdx.x] = row_scale(peak);
-            inverses[threadIdx.x] = row_inverse(scales[threadIdx.x]);
-        }
-        __syncthreads();
-    }
-    int acc[kChannels][MT] = {};
-    for (int k0 = 0; k0 < p.K; k0 += kSegment) {
-        const int len = min(kSegment, p.K - k0), seg = (len + 15) & ~15;
-        for (int i = threadIdx.x * 4; i < MT * seg; i += kFewThreads * 4) {  // seg is a multiple of 4
-            const int m = i / seg, k = i - m * seg;
-            uint32_t v = 0;
+    const int n0 = (blockIdx.x * (kOneThreads / 32) + warp) * CH;
+    if (n0 < p.N)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (m < p.M && k + j < len) {
-                    const int q = FUSED ? quantize_in(__ldg(f.x + m * f.ldx + k0 + k + j), scales[m], inverses[m])
-                                        : p.A[m * p.lda + k0 + k + j];
-                    v |= (uint32_t)(uint8_t)q << (8 * j);
-                }
-            *reinterpret_cast<uint32_t*>(tokens + i) = v;
+        for (int c = 0; c < CH; ++c) {
+            const int8_t* row = p.B + (int64_t)min(n0 + c, p.N - 1) * p.ldb;
+            for (int k = lane * 128; k < p.K; k += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + k));
         }
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    float scale = 0.0f;
+    if (NV) {
+        const bool vec = (reinterpret_cast<uintptr_t>(f.x) & 15) == 0;
+        float4 v[NV ? NV : 1];
+        uint32_t peak = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = 4 * (threadIdx.x + i * kOneThreads);
+            if (vec && k + 4 <= p.K) {
+                v[i] = __ldg(reinterpret_cast<const float4*>(f.x + k));
+            } else {
+                v[i].x = k < p.K ? __ldg(f.x + k) : 0.0f;
+                v[i].y = k + 1 < p.K ? __ldg(f.x + k + 1) : 0.0f;
+                v[i].z = k + 2 < p.K ? __ldg(f.x + k + 2) : 0.0f;
+                v[i].w = k + 3 < p.K ? __ldg(f.x + k + 3) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            peak = max(max(max(peak, abs_bits(v[i].x)), max(abs_bits(v[i].y), abs_bits(v[i].z))), abs_bits(v[i].w));
+        peak = __reduce_max_sync(0xffffffffu, peak);
+        if (lane == 0) part[warp] = peak;
+        __syncthreads();
+        scale = row_scale(__reduce_max_sync(0xffffffffu, lane < kOneThreads / 32 ? part[lane] : 0u));
+        const float inv = row_inverse(scale);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = 4 * (threadIdx.x + i * kOneThreads);
+            if (k < p.K)
+                *reinterpret_cast<char4*>(token + k) =
+                    make_char4((signed char)quantize_in(v[i].x, scale, inv), (signed char)quantize_in(v[i].y, scale, inv),
+                               (signed char)quantize_in(v[i].z, scale, inv), (signed char)quantize_in(v[i].w, scale, inv));
+        }
+    } else {
+        scale = __ldg(p.a_scale);
+    }
+    int acc[CH] = {};
+    for (int k0 = 0; k0 < p.K; k0 += kSegment) {
+        const int len = min(kSegment, p.K - k0);
+        if (!NV)
+            for (int k = threadIdx.x * 4; k < len; k += kOneThreads * 4) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (k + j < len) v |= (uint32_t)(uint8_t)p.A[k0 + k + j] << (8 * j);
+                *reinterpret_cast<uint32_t*>(token + k) = v;
+            }
         __syncthreads();
         if (n0 < p.N) {
-            const int8_t* row[kChannels];
+            const int8_t* row[CH];
 #pragma unroll
-            for (int c = 0; c < kChannels; ++c) row[c] = p.B + (int64_t)min(n0 + c, p.N - 1) * p.ldb + k0;
+            for (int c = 0; c < CH; ++c) row[c] = p.B + (int64_t)min(n0 + c, p.N - 1) * p.ldb + k0;
             const int whole = len & ~15;
-#pragma unroll 2
+#pragma unroll(8 / CH)
             for (int k = lane * 16; k < whole; k += 512) {
-                int4 w[kChannels];
+                int4 w[CH];
 #pragma unroll
-                for (int c = 0; c < kChannels; ++c) w[c] = load16<ALIGN>(row[c] + k);
+                for (int c = 0; c < CH; ++c) w[c] = load16<ALIGN>(row[c] + k);
+                const int4 t = *reinterpret_cast<const int4*>(token + k);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const int4 t = *reinterpret_cast<const int4*>(tokens + m * seg + k);
-#pragma unroll
-                    for (int c = 0; c < kChannels; ++c) acc[c][m] = dot16(w[c], t, acc[c][m]);
-                }
+                for (int c = 0; c < CH; ++c) acc[c] = dot16(w[c], t, acc[c]);
             }
             if (lane < len - whole)  // the row's last bytes, one a lane
 #pragma unroll
-                for (int c = 0; c < kChannels; ++c)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[c][m] += (int)row[c][whole + lane] * (int)tokens[m * seg + whole + lane];
+                for (int c = 0; c < CH; ++c) acc[c] += (int)row[c][whole + lane] * (int)token[whole + lane];
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int c = 0; c < kChannels; ++c)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int sum = __reduce_add_sync(0xffffffffu, acc[c][m]);
-            const int n = n0 + c;
-            if (lane == (c * MT + m) % 32 && n < p.N && m < p.M)
-                p.C[m * p.ldc + n] = i8_finish(sum, FUSED ? scales[m] : p.a_scale[m], p.b_scale[n], p.bias != nullptr,
-                                               p.bias ? p.bias[n] : 0.0f, p.relu);
-        }
+    for (int c = 0; c < CH; ++c) {
+        const int sum = __reduce_add_sync(0xffffffffu, acc[c]), n = n0 + c;
+        if (lane == c && n < p.N)
+            p.C[n] = i8_finish(sum, scale, p.b_scale[n], p.bias != nullptr, p.bias ? p.bias[n] : 0.0f, p.relu);
+    }
 }
 
-template <int MT, int ALIGN, bool FUSED>
-int launch_few(const FewArgs& f, cudaStream_t s) {
-    const unsigned grid = (unsigned)((f.p.N + kFewThreads / 32 * kChannels - 1) / (kFewThreads / 32 * kChannels));
-    const size_t smem = (size_t)MT * ((std::min(f.p.K, kSegment) + 15) & ~15);
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(gemm_i8_few_kernel<MT, ALIGN, FUSED>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, MT * kSegment) != cudaSuccess)
-        return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(gemm_i8_few_kernel) failed");
+template <int ALIGN, int NV>
+int launch_one(const OneArgs& f, cudaStream_t s) {
+    constexpr int rows = kOneThreads / 32 * CH;
     ProfScope prof(s, KID_GEMM_I8);
-    if (launch_dependent(gemm_i8_few_kernel<MT, ALIGN, FUSED>, dim3(grid), dim3(kFewThreads), smem, s, f) != cudaSuccess)
-        return set_status(JST_ERR_CUDA, "gemm_i8_few_kernel launch failed");
+    if (launch_dependent(gemm_i8_one_kernel<ALIGN, NV>, dim3((unsigned)((f.p.N + rows - 1) / rows)), dim3(kOneThreads), 0,
+                         s, f) != cudaSuccess)
+        return set_status(JST_ERR_CUDA, "gemm_i8_one_kernel launch failed");
     return JST_OK;
 }
 
-template <bool FUSED>
-int run_few(const FewArgs& f, cudaStream_t s) {
+template <int NV>
+int run_one_nv(const OneArgs& f, cudaStream_t s) {
     const bool al = (reinterpret_cast<uintptr_t>(f.p.B) & 15) == 0 && (f.p.N == 1 || (f.p.ldb & 15) == 0);
-    if (f.p.M == 1) return al ? launch_few<1, 16, FUSED>(f, s) : launch_few<1, 1, FUSED>(f, s);
-    if (f.p.M == 2) return al ? launch_few<2, 16, FUSED>(f, s) : launch_few<2, 1, FUSED>(f, s);
-    if (f.p.M <= 4) return al ? launch_few<4, 16, FUSED>(f, s) : launch_few<4, 1, FUSED>(f, s);
-    return al ? launch_few<8, 16, FUSED>(f, s) : launch_few<8, 1, FUSED>(f, s);
+    return al ? launch_one<16, NV>(f, s) : launch_one<1, NV>(f, s);
+}
+
+// x: the token in fp32, K <= kSegment; or null, and the token is in A.
+int run_one(const I8Args& p, const float* x, cudaStream_t s) {
+    const OneArgs f{p, x};
+    if (!x) return run_one_nv<0>(f, s);
+    return p.K <= 1024 ? run_one_nv<1>(f, s) : p.K <= 4096 ? run_one_nv<4>(f, s) : run_one_nv<8>(f, s);
 }
 
 // K == 0: every sum is 0.
@@ -228,9 +286,25 @@ int check_quantize(const float* x, int64_t ldx, int rows, int cols, const int8_t
 
 int run_quantize(const float* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scale, cudaStream_t s) {
     if (rows == 0) return set_status(JST_OK, nullptr);
+    const bool vec = ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && (rows == 1 || (ldx & 3) == 0)) &&
+                     ((reinterpret_cast<uintptr_t>(q) & 3) == 0 && (rows == 1 || (ldq & 3) == 0));
+    // Groups of four values: few rows get a thread for each (a row's latency is
+    // what counts), many rows up to eight a thread.
+    const int groups = (cols + 3) / 4, most = rows < 2 * sm_count() ? 1024 : 256;
+    int threads = std::min(most, std::max(32, (groups + 31) / 32 * 32)), nv = (groups + threads - 1) / threads;
+    if (nv > 8) {
+        threads = 1024;
+        nv = (groups + threads - 1) / threads;
+    }
+    auto go = [&](auto kernel) { return launch_dependent(kernel, dim3((unsigned)rows), dim3(threads), 0, s, x, ldx, cols, q, ldq, scale); };
     {
         ProfScope prof(s, KID_QUANT);
-        quantize_rows_kernel<<<(unsigned)rows, kQuantThreads, 0, s>>>(x, ldx, cols, q, ldq, scale);
+        const cudaError_t e = nv <= 1   ? (vec ? go(quantize_rows_kernel<1, true>) : go(quantize_rows_kernel<1, false>))
+                              : nv <= 2 ? (vec ? go(quantize_rows_kernel<2, true>) : go(quantize_rows_kernel<2, false>))
+                              : nv <= 4 ? (vec ? go(quantize_rows_kernel<4, true>) : go(quantize_rows_kernel<4, false>))
+                              : nv <= 8 ? (vec ? go(quantize_rows_kernel<8, true>) : go(quantize_rows_kernel<8, false>))
+                                        : (vec ? go(quantize_rows_kernel<0, true>) : go(quantize_rows_kernel<0, false>));
+        if (e != cudaSuccess) return set_status(JST_ERR_CUDA, "quantize_rows launch failed");
     }
     return launched("quantize_rows launch failed");
 }
@@ -250,15 +324,8 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     return JST_OK;
 }
 
-// Up to kFew tokens the product is a read of the weight, and dp4a keeps up
-// with it; from there on the tensor cores' work a byte of weight is free.
-constexpr int kFew = 8;
-// Up to so many values every block of the product quantises the tokens itself;
-// more are quantised once, by a launch of their own.
-constexpr int64_t kFusedValues = 16384;
-
 int run_gemm_i8(const I8Args& p, cudaStream_t s) {
-    const int rc = p.K == 0 ? run_empty(p, s) : p.M <= kFew ? run_few<false>({p, nullptr, 0}, s) : gemm_i8_tc_run(p, s);
+    const int rc = p.K == 0 ? run_empty(p, s) : p.M == 1 ? run_one(p, nullptr, s) : gemm_i8_tc_run(p, s);
     return rc ? rc : launched("gemm_i8 launch failed");
 }
 
@@ -310,8 +377,8 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     I8Args p{M, N, K, nullptr, 0, w, ldw, nullptr, w_scale, (epilogue & JST_EPI_BIAS) ? bias : nullptr,
              (epilogue & JST_EPI_RELU) ? 1 : 0, y, ldy};
-    if (K == 0 || (M <= kFew && (int64_t)M * K <= kFusedValues)) {
-        rc = K == 0 ? run_empty(p, s) : run_few<true>({p, x, ldx}, s);
+    if (K == 0 || (M == 1 && K <= kSegment)) {
+        rc = K == 0 ? run_empty(p, s) : run_one(p, x, s);
         return rc ? rc : launched("linear_i8 launch failed");
     }
     const int64_t ldq = ((int64_t)K + 15) / 16 * 16;

@@ -413,9 +413,6 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(const ScanA
 //            round's loads in flight while this one is folded and written.
 // Every order is fixed, so results repeat bit for bit.
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // V channels' pair in shared memory.
 template <int V>
 struct __align__(8 * V) Pair {
@@ -424,9 +421,7 @@ struct __align__(8 * V) Pair {
 // Store to the same place in block `rank` of the cluster; its barrier counts the bytes as they arrive.
 template <int V>
 __device__ __forceinline__ void send(Pair<V>* to, uint64_t* bar, int rank, const Pair<V>& v) {
-    uint32_t at, at_bar;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(to)), "r"(rank));
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_bar) : "r"(ptx::smem_u32(bar)), "r"(rank));
+    const uint32_t at = ptx::cluster_addr(ptx::smem_u32(to), rank), at_bar = ptx::cluster_addr(ptx::smem_u32(bar), rank);
     if constexpr (V == 2)
         asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at),
                      "r"(__float_as_uint(v.A.v[0])), "r"(__float_as_uint(v.A.v[1])), "r"(__float_as_uint(v.B.v[0])),
@@ -459,8 +454,8 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
             gave_up = 0;
             ptx::fence_barrier_init();
         }
-        cluster_arrive();  // every block's barriers are set up before any block sends
-        cluster_wait();
+        ptx::cluster_arrive();  // every block's barriers are set up before any block sends
+        ptx::cluster_wait();
     }
     uint32_t round = 0;
     for (int64_t base = 0; base < p.seq; base += round_steps, ++round) {
@@ -494,7 +489,7 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
                 // only after that other has sent the round between: it has read them.
                 for (int q = 0; q < C; ++q) send(&blocks[parity][rank][lane], &arrived[parity], q, run);
             }
-            ptx::mbar_wait(&arrived[parity], (round >> 1) & 1, &gave_up);
+            ptx::mbar_wait<true>(&arrived[parity], (round >> 1) & 1, &gave_up);
             for (int q = 0; q < C; ++q) {
                 if (q == rank) e = carry;
                 const Pair<V> f = blocks[parity][q][lane];
@@ -519,8 +514,8 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
     if (rank == 0 && warp == 0) w.set_state(BWD ? p.dh0 : p.h_n, carry);
     if (C > 1) {
         if (threadIdx.x == 0 && gave_up) atomicOr(p.err, gave_up);
-        cluster_arrive();  // nobody leaves while another could still send to it
-        cluster_wait();
+        ptx::cluster_arrive();  // nobody leaves while another could still send to it
+        ptx::cluster_wait();
     }
 }
 
