@@ -32,7 +32,6 @@
 
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <cstdint>
 #include <mutex>
 
@@ -56,8 +55,8 @@ struct Cfg {
     static constexpr uint32_t R_BYTES = BM * BK;
     static constexpr uint32_t S_BYTES = BN_ * BK;
     static constexpr uint32_t STAGE_BYTES = R_BYTES + S_BYTES;
-    static constexpr uint32_t STG_OFF = STAGES_ * STAGE_BYTES;  // a 32 x 32 block per epilogue warp
-    static constexpr uint32_t TAB_OFF = STG_OFF + 8 * 4096;     // a scale and bias table per epilogue warp
+    static constexpr uint32_t STG_OFF = STAGES_ * STAGE_BYTES;  // two 32 x 32 blocks per epilogue warp
+    static constexpr uint32_t TAB_OFF = STG_OFF + 8 * 8192;     // a scale and bias table per epilogue warp
     static constexpr uint32_t BAR_OFF = TAB_OFF + 8 * 256;
     static constexpr uint32_t SMEM_BYTES = BAR_OFF + 256 + 768 /*from 256- to 1024-byte alignment*/;
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
@@ -92,34 +91,47 @@ __device__ __forceinline__ void tile_at(int t, const Params& p, int bn, int* r0,
 
 // One epilogue warp's part of a tile: wait for the accumulator at `acc`, drain
 // TMEM lane quadrant q's 32-column blocks half, half + 2, ..., release() the
-// accumulator after the last read of it, and write C.  False: a wait gave up.
-template <int BN, class Release>
+// accumulator after the last read of it, and write C.  The blocks' scales are
+// on their way while the accumulator is not complete, and a block is staged
+// while the one before it is being stored (STAGED places a warp).  False: a wait gave up.
+template <int BN, int STAGED, class Release>
 __device__ __forceinline__ bool drain_tile(const Params& p, const CUtensorMap& tm_c, uint32_t acc, uint64_t* complete,
                                            uint32_t phase, volatile uint32_t* err, int r0, int s0, int q, int half,
-                                           uint8_t* blk, float* tab, bool& stored, Release release) {
+                                           uint8_t* stage, float* tab, uint32_t& stores, Release release) {
+    constexpr int MINE = (BN / 32 + 1) / 2;  // blocks of a warp
     const int lane = threadIdx.x & 31;
     const int row = r0 + q * 32 + lane;
     const float rs = row < p.R ? __ldg(p.r_scale + row) : 0.0f;
+    float scale[MINE], bias[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int col = min(s0 + (half + 2 * i) * 32 + lane, p.S - 1);
+        scale[i] = __ldg(p.s_scale + col);
+        bias[i] = p.bias ? __ldg(p.bias + col) : 0.0f;
+    }
     int okw = 0;
     if (lane == 0) okw = ptx::mbar_wait(complete, phase, err) && *err == 0;
     if (!__shfl_sync(0xffffffffu, okw, 0)) return false;
     ptx::tc_fence_after();
-    const int nblk = min((BN + 31) / 32, (p.S - s0 + 31) / 32);
+    const int nblk = min(BN / 32, (p.S - s0 + 31) / 32);
     const int last = nblk - 1 - ((nblk - 1 - half) & 1);
     if (last < 0) {  // a warp without a block still releases the accumulator
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) release();
     }
-#pragma unroll 1
-    for (int c = half; c < nblk; c += 2) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int c = half + 2 * i;
+        if (c >= nblk) break;
         const int col0 = s0 + c * 32;
-        const int col = min(col0 + lane, p.S - 1);
-        __syncwarp();  // the previous block's readers of the tables are done
-        tab[lane] = __ldg(p.s_scale + col);
-        tab[32 + lane] = p.bias ? __ldg(p.bias + col) : 0.0f;
+        uint8_t* blk = stage + (stores % STAGED) * 4096;
         uint32_t r[32];
         ptx::tmem_ld_32x32b_x32(acc + ((uint32_t)(q * 32) << 16) + c * 32, r);
+        __syncwarp();  // the previous block's readers of the tables are done
+        tab[lane] = scale[i];
+        tab[32 + lane] = bias[i];
+        if (p.tma_store && lane == 0) ptx::bulk_wait_read<STAGED - 1>();  // the store that used `blk` has read it
         ptx::tmem_ld_wait();
         if (c == last) {
             ptx::tc_fence_before();
@@ -127,11 +139,11 @@ __device__ __forceinline__ bool drain_tile(const Params& p, const CUtensorMap& t
             if (lane == 0) release();
         }
         __syncwarp();
+        const bool hb = p.bias != nullptr;
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
             const float4 sc = *reinterpret_cast<const float4*>(tab + j);
             const float4 bi = *reinterpret_cast<const float4*>(tab + 32 + j);
-            const bool hb = p.bias != nullptr;
             r[j + 0] = __float_as_uint(i8_finish((int)r[j + 0], rs, sc.x, hb, bi.x, p.relu));
             r[j + 1] = __float_as_uint(i8_finish((int)r[j + 1], rs, sc.y, hb, bi.y, p.relu));
             r[j + 2] = __float_as_uint(i8_finish((int)r[j + 2], rs, sc.z, hb, bi.z, p.relu));
@@ -139,8 +151,6 @@ __device__ __forceinline__ bool drain_tile(const Params& p, const CUtensorMap& t
         }
         if (p.tma_store) {
             if (r0 + q * 32 < p.R) {  // the box parts past R or S are not written
-                if (lane == 0 && stored) ptx::bulk_wait_read<0>();
-                __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     *reinterpret_cast<uint4*>(blk + lane * 128 + ((j ^ (lane & 7)) << 4)) =
@@ -151,20 +161,21 @@ __device__ __forceinline__ bool drain_tile(const Params& p, const CUtensorMap& t
                     ptx::tma_store_3d(&tm_c, blk, col0, r0 + q * 32, 0);
                     ptx::bulk_commit();
                 }
-                stored = true;
+                ++stores;
             }
         } else {  // transpose through shared memory: one 128-byte row segment a store
-            __syncwarp();
 #pragma unroll
             for (int j = 0; j < 32; ++j)  // word j of row `lane` at j ^ lane: no bank conflicts either way
                 reinterpret_cast<uint32_t*>(blk)[lane * 32 + (j ^ lane)] = r[j];
             __syncwarp();
-            if (col0 + lane < p.S)
-                for (int j = 0; j < 32; ++j)
-                    if (r0 + q * 32 + j < p.R)
-                        p.C[(int64_t)(r0 + q * 32 + j) * p.ldc + col0 + lane] =
-                            __uint_as_float(reinterpret_cast<uint32_t*>(blk)[j * 32 + (lane ^ j)]);
-            __syncwarp();
+            if (col0 + lane < p.S) {
+                float* out = p.C + (int64_t)(r0 + q * 32) * p.ldc + col0 + lane;
+                const int rows = min(32, p.R - (r0 + q * 32));
+#pragma unroll 8
+                for (int j = 0; j < rows; ++j)
+                    out[j * p.ldc] = __uint_as_float(reinterpret_cast<uint32_t*>(blk)[j * 32 + (lane ^ j)]);
+            }
+            ++stores;
         }
     }
     return true;
@@ -266,19 +277,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else {
         const int q = warp & 3;            // TMEM lane quadrant this warp may access
         const int half = (warp - 2) >> 2;  // 0: even 32-column blocks, 1: odd
-        uint8_t* blk = smem + C::STG_OFF + (warp - 2) * 4096;
+        uint8_t* blk = smem + C::STG_OFF + (warp - 2) * 8192;
         float* tab = reinterpret_cast<float*>(smem + C::TAB_OFF + (warp - 2) * 256);  // [32] scale, [32] bias
-        bool stored = false;
+        uint32_t stores = 0;  // blocks staged by this warp
         int i = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x, ++i) {
             const int buf = i & 1;
             int r0, s0;
             tile_at(t, p, BN, &r0, &s0);
-            if (!drain_tile<BN>(p, tm_c, tmem_base + buf * C::ACC_COLS, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
-                                blk, tab, stored, [&] { ptx::mbar_arrive(&acce_bar[buf]); }))
+            if (!drain_tile<BN, 2>(p, tm_c, tmem_base + buf * C::ACC_COLS, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
+                                blk, tab, stores, [&] { ptx::mbar_arrive(&acce_bar[buf]); }))
                 break;
         }
-        if (lane == 0 && stored) ptx::bulk_wait_all();  // C is written before the CTA exits
+        if (lane == 0 && stores) ptx::bulk_wait_all();  // C is written before the CTA exits
     }
 
     ptx::tc_fence_before();
@@ -305,7 +316,7 @@ struct PairCfg {
     static constexpr uint32_t HALF_BYTES = BM * BK;  // 128 rows of R, 128 rows of S
     static constexpr uint32_t STAGE_BYTES = 2 * HALF_BYTES;
     static constexpr uint32_t STG_OFF = STAGES * STAGE_BYTES;
-    static constexpr uint32_t TAB_OFF = STG_OFF + 8 * 4096;
+    static constexpr uint32_t TAB_OFF = STG_OFF + 8 * 4096;  // one 32 x 32 block a warp: a sixth stage is worth more (8192^3: 365 us; five and two blocks 384)
     static constexpr uint32_t BAR_OFF = TAB_OFF + 8 * 256;
     static constexpr uint32_t SMEM_BYTES = BAR_OFF + 256 + 768;
     static_assert(SMEM_BYTES <= 227 * 1024 && (2 * STAGES + 5) * 8 + 8 <= 256, "shared memory per CTA");
@@ -425,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int half = (warp - 2) >> 2;
         uint8_t* blk = smem + C::STG_OFF + (warp - 2) * 4096;
         float* tab = reinterpret_cast<float*>(smem + C::TAB_OFF + (warp - 2) * 256);
-        bool stored = false;
+        uint32_t stores = 0;  // blocks staged by this warp
         int i = 0;
         for (int t = pair; t < total; t += pairs, ++i) {
             const int buf = i & 1;
@@ -433,11 +444,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             pair_tile_at(t, p, &r0, &s0);
             r0 += rank * BM;
             const uint32_t drained = ptx::cluster_addr(ptx::smem_u32(&acce_bar[buf]), 0);
-            if (!drain_tile<C::BN>(p, tm_c, tmem_base + buf * C::BN, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
-                                   blk, tab, stored, [&] { ptx::mbar_arrive_cluster(drained); }))
+            if (!drain_tile<C::BN, 1>(p, tm_c, tmem_base + buf * C::BN, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
+                                   blk, tab, stores, [&] { ptx::mbar_arrive_cluster(drained); }))
                 break;
         }
-        if (lane == 0 && stored) ptx::bulk_wait_all();
+        if (lane == 0 && stores) ptx::bulk_wait_all();
         __syncwarp();
     }
 
@@ -793,21 +804,26 @@ static int run_tokens(const I8Args& a, cudaStream_t s) {
 
 static int run_aligned(const I8Args& a, cudaStream_t s) {
     if (a.M <= 64) return run_tokens(a, s);
-    // Waves of tiles times what a tile costs a k-slab: the 128 token rows that
-    // it stages whatever its width, and its own BN rows.
-    const int64_t rows = (a.M + BM - 1) / BM, sms = sm_count();
-    int bn = 256;
+    // The tile by what it is expected to take, in ns measured on a B200: a k-slab
+    // (8192^3: 384 us in pairs, 602 and 1055 in tiles of 128 and 64 columns) or,
+    // where K is short, the epilogue (8192 x 8192 x 512: 93, 66, 93) of a tile,
+    // times the waves of tiles, and one of each at the ends.  (256 x 8192 x 8192:
+    // 31.5, 25.1, 42.1; 128 x 8192 x 8192: 39.9, 25.1, 23.4; 2048^3: 19.4, 16.4,
+    // 23.9; 3000^3: 25.8, 36.2, 62.8.)
+    const struct { int rows, cols, slots, slab_ns, epilogue_ns; } kinds[] = {
+        {2 * BM, 256, sm_count() / 2, 410, 6500}, {BM, 128, sm_count(), 336, 2400}, {BM, 64, sm_count(), 294, 1650}};
+    int bn = 0;
     int64_t best = INT64_MAX;
-    for (int n : {256, 128, 64}) {
-        const int64_t waves = (rows * ((a.N + n - 1) / n) + sms - 1) / sms, cost = waves * (n + 64);
+    for (const auto& k : kinds) {
+        const int64_t tiles = (int64_t)((a.M + k.rows - 1) / k.rows) * ((a.N + k.cols - 1) / k.cols);
+        const int64_t waves = (tiles + k.slots - 1) / k.slots, slabs = (int64_t)((a.K + BK - 1) / BK) * k.slab_ns;
+        const int64_t cost = (waves - 1) * std::max<int64_t>(slabs, k.epilogue_ns) + slabs + k.epilogue_ns;
         if (cost < best) {
             best = cost;
-            bn = n;
+            bn = k.cols;
         }
     }
-    const char* e = getenv("JST_PAIR");
-    const bool pair = e && atoi(e);
-    if (pair) bn = 256;
+    const bool pair = bn == 256;
     Params p{};
     p.R = a.M; p.S = a.N; p.K = a.K;
     p.C = a.C; p.ldc = a.ldc;
@@ -824,7 +840,6 @@ static int run_aligned(const I8Args& a, cudaStream_t s) {
     p.tma_store = (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 && (a.ldc & 3) == 0 &&
                   make_map(&mc, a.C, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, a.N, a.M, a.ldc, 32);
     if (pair) return launch_pair(mr, ms, mc, p, s);
-    if (bn == 256) return launch<Cfg<256, 4>>(mr, ms, mc, p, s);
     if (bn == 128) return launch<Cfg<128, 5>>(mr, ms, mc, p, s);
     return launch<Cfg<64, 6>>(mr, ms, mc, p, s);
 }

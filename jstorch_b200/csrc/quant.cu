@@ -14,7 +14,7 @@
 namespace jst {
 namespace {
 
-// q = x / s to the nearest integer, ties to even, where s = max|x| / 127 > 0.
+// q = x / s to the nearest integer, ties to even, where s = max|x| * (1 / 127) > 0.
 // x * (1 / s) is within a few 2^-24 of the quotient, so only a value within
 // 2^-12 of a half can round to another integer than the quotient does; those
 // (one in two thousand) divide in 64 bits, which separates every quotient of
@@ -32,7 +32,7 @@ __device__ __forceinline__ int quantize(float x, float s, float inv) {
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 __device__ __forceinline__ float row_scale(uint32_t peak) {
-    return peak < 0x7f800000u ? __fdiv_rn(__uint_as_float(peak), 127.0f) : __uint_as_float(0x7fffffffu);
+    return peak < 0x7f800000u ? __fmul_rn(__uint_as_float(peak), 1.0f / 127.0f) : __uint_as_float(0x7fffffffu);
 }
 // 1 / s, or 0 where the row quantises to zeros (s is 0 or NaN).
 __device__ __forceinline__ float row_inverse(float s) { return s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f; }
