@@ -30,6 +30,15 @@ def test_sizes_and_alignments(n, shift):
     assert bool((out[:1] == 7).all()) and bool((out[1 + n:] == 7).all())
 
 
+@pytest.mark.parametrize("n,shift", [(1212416, 0), (1300001, 0), (2500003, 1)])
+def test_many_elements(n, shift):
+    import torch
+
+    import jstorch_b200
+    x = np.random.default_rng(n).standard_normal(n + shift).astype(np.float32)
+    _equal(jstorch_b200.dropout(torch.from_numpy(x).cuda()[shift:], 0.6, SEED, OFFSET), x[shift:], 0.6)
+
+
 @pytest.mark.parametrize("p", [0.0, 2.0 ** -33, 0.1, 0.5, 0.9, 1 - 2.0 ** -24, 1.0])
 def test_probabilities(p):
     import torch
