@@ -143,7 +143,8 @@ __device__ __forceinline__ float at_most(float x, float hi) {
 }
 
 // z = 1 / (1 + e) and 1 - z = e z with e = exp(-a): neither loses digits where
-// it is small.  a is kept within [-87, 127], where e is a number and z is
+// it is small.  The reciprocal takes one Newton step: its ulp leans to one side,
+// and a state that is remembered for a thousand steps would add it up.  a is kept within [-87, 127], where e is a number and z is
 // positive: below, z is held at 2^-126 (1.65e-38), which a state's share of
 // the next one cannot show beside anything but 0.
 template <int V>
@@ -151,8 +152,8 @@ __device__ __forceinline__ void gate(const F<V>& a, F<V>& z, F<V>& rest) {
     F<V> x;
 #pragma unroll
     for (int i = 0; i < V; ++i) x.v[i] = at_most(at_least(a.v[i], -87.0f), 127.0f);
-    const F<V> e = exp_minus(x);
-    z = reciprocal(e + all<V>(1.0f));
+    const F<V> e = exp_minus(x), d = e + all<V>(1.0f), r = reciprocal(d);
+    z = fma(r, fma(-d, r, all<V>(1.0f)), r);
     rest = e * z;
 }
 
