@@ -194,50 +194,44 @@ def check_last() -> None:
     check(load().jst_get_last_status())
 
 
-def is_f32(x, device=None) -> bool:
-    """Whether x is a float32 CUDA tensor (on `device`, where one is given)."""
-    import torch
-
-    return isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.is_cuda and (device is None or x.device == device)
-
-
-def require_f32(x, name: str) -> None:
-    """Raise unless x is a float32 CUDA tensor."""
+def require_f32(x, name: str) -> int:
+    """The device index of x; raises unless x is a float32 CUDA tensor."""
     import torch
 
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if x.dtype is not torch.float32:
         raise TypeError(f"{name} must be float32 (got {x.dtype})")
-    if not x.is_cuda:
+    index = x.get_device()
+    if index < 0 or not x.is_cuda:
         raise ValueError(f"{name} must live on a CUDA device")
+    return index
 
 
-def empty(like, shape, stream, dtype=None):
-    """An uninitialised tensor on like's device, of its type by default, that
-    belongs to `stream`: memory that torch's allocator reuses in another
-    stream's order could still be in use there when `stream` writes it."""
+def empty(like, shape, stream):
+    """An uninitialised tensor on like's device, of its type, that belongs to
+    `stream`: memory that torch's allocator reuses in another stream's order
+    could still be in use there when `stream` writes it."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype) if dtype is not None else like.new_empty(shape)
+        return like.new_empty(shape)
     import torch
 
     with torch.cuda.stream(stream):
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(shape)
 
 
-def call(device, stream, function, *args) -> None:
-    """function(*args, stream handle) with `device` current, on `stream` (by
-    default torch's current stream of the device); raises on a status."""
+def call(index: int, stream, function, *args) -> None:
+    """function(*args, stream handle) with device `index` current, on `stream`
+    (by default torch's current stream of the device); raises on a status."""
     import torch
 
-    index = device.index
     if stream is None:
         handle = torch._C._cuda_getCurrentRawStream(index)  # a Stream object costs 2 us a call
-    elif stream.device != device:
-        raise ValueError(f"stream belongs to {stream.device}, the tensors to {device}")
+    elif stream.device.index != index:
+        raise ValueError(f"stream belongs to {stream.device}, the tensors to cuda:{index}")
     else:
         handle = stream.cuda_stream
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         status = function(*args, handle)
     else:
         with torch.cuda.device(index):

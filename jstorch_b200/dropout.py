@@ -11,7 +11,8 @@ from . import _lib
 def _rows(x, name: str):
     """(rows, cols, pitch) of x as a row-major matrix; contiguous tensors are one row."""
     if x.is_contiguous():
-        return 1, x.numel(), x.numel()
+        n = x.numel()
+        return 1, n, n
     shape, stride = x.shape, x.stride()
     cols = shape[-1]
     if cols > 1 and stride[-1] != 1:
@@ -40,27 +41,27 @@ def dropout(x, p: float, seed: int, offset: int = 0, *, step=None, out=None, str
     that advances it draws a new mask at every replay.  out may be x itself.
     Runs asynchronously on `stream` (default: torch's current stream).
     """
-    import torch
-
-    _lib.require_f32(x, "x")
+    index = _lib.require_f32(x, "x")
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p must be in [0, 1] (got {p})")
     if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
         raise ValueError("seed and offset must be 64-bit unsigned integers")
-    if step is not None and (step.dtype != torch.int64 or step.numel() != 1 or step.device != x.device):
-        raise ValueError("step must be a one-element int64 tensor on x's device")
+    if step is not None:
+        import torch
+
+        if step.dtype is not torch.int64 or step.numel() != 1 or step.get_device() != index:
+            raise ValueError("step must be a one-element int64 tensor on x's device")
+        step = step.data_ptr()
     if out is None:
         out = _lib.empty(x, x.shape, stream)
-    else:
-        _lib.require_f32(out, "out")
-        if out.shape != x.shape or out.device != x.device:
-            raise ValueError(f"out must be a float32 tensor of shape {tuple(x.shape)} on x's device")
+    elif _lib.require_f32(out, "out") != index or out.shape != x.shape:
+        raise ValueError(f"out must be a float32 tensor of shape {tuple(x.shape)} on x's device")
     rows, cols, ldx = _rows(x, "x")
     rows_o, cols_o, ldy = _rows(out, "out")
     if (rows, cols) != (rows_o, cols_o):  # one of the two has gaps: the other has rows of the same length without any
         rows, cols = max((rows, cols), (rows_o, cols_o))
         ldx = cols if x.is_contiguous() else ldx
         ldy = cols if out.is_contiguous() else ldy
-    _lib.call(x.device, stream, _lib.load().jst_dropout, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, cols, float(p), seed,
-              offset, step.data_ptr() if step is not None else None)
+    _lib.call(index, stream, _lib.load().jst_dropout, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, cols, p, seed, offset,
+              step)
     return out

@@ -9,47 +9,49 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from . import _lib
 
 
-def _int8_rows(x, name: str):
-    """(rows, cols, pitch) of a 2-D int8 CUDA tensor whose columns are adjacent."""
-    import torch
-
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if x.dtype != torch.int8:
-        raise TypeError(f"{name} must be int8 (got {x.dtype})")
-    if not x.is_cuda:
-        raise ValueError(f"{name} must live on a CUDA device")
-    return _matrix(x, name)
-
-
 def _matrix(x, name: str):
+    """(rows, cols, pitch) of a 2-D tensor whose columns are adjacent."""
     if x.dim() != 2:
         raise ValueError(f"{name} must be 2-D")
     rows, cols = x.shape
+    if x.is_contiguous():
+        return rows, cols, cols or 1
     pitch, unit = x.stride()
     if (cols > 1 and unit != 1) or (rows > 1 and pitch < cols):
         raise ValueError(f"{name}: unsupported strides {tuple(x.stride())} for shape {tuple(x.shape)}")
     return rows, cols, pitch if rows > 1 else max(cols, 1)
 
 
-def _vector(v, name: str, n: int, device):
-    if not _lib.is_f32(v, device) or v.shape != (n,) or (n > 1 and v.stride(0) != 1):
-        _lib.require_f32(v, name)
-        raise ValueError(f"{name} must be a contiguous float32 tensor with {n} elements on {device}")
+def _require_i8(x, name: str) -> int:
+    """The device index of x; raises unless x is an int8 CUDA tensor."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dtype is not torch.int8:
+        raise TypeError(f"{name} must be int8 (got {x.dtype})")
+    index = x.get_device()
+    if index < 0 or not x.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device")
+    return index
+
+
+def _vector(v, name: str, n: int, index: int):
+    """Address of n adjacent float32 values on device `index`."""
+    if _lib.require_f32(v, name) != index or v.shape != (n,) or not v.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor with {n} elements on cuda:{index}")
     return v.data_ptr()
 
 
-def _output(out, like, M: int, N: int, device, stream):
+def _output(out, like, M: int, N: int, index: int, stream):
+    """(out, its pitch): a float32 [M, N] tensor, made where none is given."""
     if out is None:
-        import torch
-
-        return _lib.empty(like, (M, N), stream, torch.float32), N
-    _lib.require_f32(out, "out")
-    if out.shape != (M, N) or out.device != device:
-        raise ValueError(f"out must be a float32 tensor of shape {(M, N)} on {device}")
+        return _lib.empty(like, (M, N), stream), N or 1
+    if _lib.require_f32(out, "out") != index or out.shape != (M, N):
+        raise ValueError(f"out must be a float32 tensor of shape {(M, N)} on cuda:{index}")
     return out, _matrix(out, "out")[2]
 
 
@@ -60,14 +62,12 @@ def quantize_rows(x, *, stream=None):
     at multiples of 16 bytes (q is a view when x has other widths), as
     gemm_i8 reads them in place.
     """
-    import torch
-
-    _lib.require_f32(x, "x")
+    index = _lib.require_f32(x, "x")
     rows, cols, ldx = _matrix(x, "x")
     pitch = max((cols + 15) // 16 * 16, 16)
-    held = _lib.empty(x, (rows, pitch), stream, torch.int8)
     scale = _lib.empty(x, (rows,), stream)
-    _lib.call(x.device, stream, _lib.load().jst_quantize_rows_i8, x.data_ptr(), ldx, rows, cols, held.data_ptr(), pitch,
+    held = _lib.empty(x, (rows, pitch // 4), stream).view(torch.int8)
+    _lib.call(index, stream, _lib.load().jst_quantize_rows_i8, x.data_ptr(), ldx, rows, cols, held.data_ptr(), pitch,
               scale.data_ptr())
     return held[:, :cols], scale
 
@@ -86,22 +86,19 @@ def gemm_i8(a, w, a_scale, w_scale, out=None, *, bias=None, relu: bool = False, 
     float32 [M, N] (a pitch is allowed).  Runs asynchronously on `stream`
     (default: torch's current stream).
     """
-    M, K, lda = _int8_rows(a, "a")
-    N, Kw, ldw = _int8_rows(w, "w")
+    index = _require_i8(a, "a")
+    if _require_i8(w, "w") != index:
+        raise ValueError("a and w must live on one device")
+    M, K, lda = _matrix(a, "a")
+    N, Kw, ldw = _matrix(w, "w")
     if K != Kw:
         raise ValueError(f"gemm_i8 shape mismatch: a is [{M}, {K}], w is [{N}, {Kw}]")
-    if w.device != a.device:
-        raise ValueError("a and w must live on one device")
-    d = _lib.GemmI8Desc()
-    d.M, d.N, d.K = M, N, K
-    d.A, d.lda, d.B, d.ldb = a.data_ptr(), lda, w.data_ptr(), ldw
-    d.a_scale = _vector(a_scale, "a_scale", M, a.device)
-    d.b_scale = _vector(w_scale, "w_scale", N, a.device)
-    d.bias = _vector(bias, "bias", N, a.device) if bias is not None else None
-    d.epilogue = (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0)
-    out, d.ldc = _output(out, a, M, N, a.device, stream)
+    d = _lib.GemmI8Desc(M, N, K, a.data_ptr(), lda, w.data_ptr(), ldw, _vector(a_scale, "a_scale", M, index),
+                        _vector(w_scale, "w_scale", N, index), _vector(bias, "bias", N, index) if bias is not None else None,
+                        (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0))
+    out, d.ldc = _output(out, a_scale, M, N, index, stream)
     d.C = out.data_ptr()
-    _lib.call(a.device, stream, _run_desc, d)
+    _lib.call(index, stream, _run_desc, d)
     return out
 
 
@@ -110,16 +107,16 @@ def linear_i8(x, w, w_scale, out=None, *, bias=None, relu: bool = False, stream=
     w [N, K] int8 with w_scale [N] (quantize_rows of the weight), out float32
     [M, N].  The same result as the two calls, in fewer passes.
     """
-    _lib.require_f32(x, "x")
+    index = _lib.require_f32(x, "x")
+    if _require_i8(w, "w") != index:
+        raise ValueError("x and w must live on one device")
     M, K, ldx = _matrix(x, "x")
-    N, Kw, ldw = _int8_rows(w, "w")
+    N, Kw, ldw = _matrix(w, "w")
     if K != Kw:
         raise ValueError(f"linear_i8 shape mismatch: x is [{M}, {K}], w is [{N}, {Kw}]")
-    if w.device != x.device:
-        raise ValueError("x and w must live on one device")
-    ws = _vector(w_scale, "w_scale", N, x.device)
-    b = _vector(bias, "bias", N, x.device) if bias is not None else None
-    out, ldy = _output(out, x, M, N, x.device, stream)
-    _lib.call(x.device, stream, _lib.load().jst_linear_i8, x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, ws, N, b,
+    scale = _vector(w_scale, "w_scale", N, index)
+    b = _vector(bias, "bias", N, index) if bias is not None else None
+    out, ldy = _output(out, x, M, N, index, stream)
+    _lib.call(index, stream, _lib.load().jst_linear_i8, x.data_ptr(), ldx, M, K, w.data_ptr(), ldw, scale, N, b,
               (_lib.EPI_BIAS if bias is not None else 0) | (_lib.EPI_RELU if relu else 0), out.data_ptr(), ldy)
     return out

@@ -218,14 +218,13 @@ class GRU(_LayerDropout):
 CANDIDATES = {"tanh": 0, "identity": 1}  # JST_SCAN_* (include/jstorch_scan.h)
 
 
-def _step_rows(x, name: str, shape, device) -> int:
+def _step_rows(x, name: str, shape, index: int) -> int:
     """Row pitch of a float32 tensor [seq, batch, cols] whose rows are equally far apart."""
-    if not _lib.is_f32(x, device) or x.shape != shape:
-        _lib.require_f32(x, name)
-        raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)} on {device}")
-    if x.is_contiguous():
-        return shape[2]
+    if _lib.require_f32(x, name) != index or x.shape != shape:
+        raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)} on cuda:{index}")
     seq, batch, cols = shape
+    if x.is_contiguous():
+        return cols
     s0, s1, s2 = x.stride()
     pitch = s1 if batch > 1 else (s0 if seq > 1 else cols)
     if (cols > 1 and s2 != 1) or pitch < cols or (seq > 1 and batch > 1 and s0 != batch * s1):
@@ -233,32 +232,30 @@ def _step_rows(x, name: str, shape, device) -> int:
     return pitch
 
 
-def _state(h, name: str, shape, device):
-    """Address of a contiguous float32 tensor of `shape`, None of None."""
-    if h is None:
-        return None
-    if not _lib.is_f32(h, device) or h.shape != shape or not h.is_contiguous():
-        _lib.require_f32(h, name)
-        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {shape} on {device}")
+def _state(h, name: str, batch: int, hidden: int, index: int) -> int:
+    """Address of a contiguous float32 tensor [batch, hidden]."""
+    if _lib.require_f32(h, name) != index or h.shape != (batch, hidden) or not h.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {(batch, hidden)} on cuda:{index}")
     return h.data_ptr()
 
 
 def _scan_args(gates, h0, lengths, candidate):
-    """(device, seq, batch, hidden, gate pitch, h0, lengths, candidate), the last three as the C entry points take them."""
-    import torch
-
-    _lib.require_f32(gates, "gates")
+    """(device index, seq, batch, hidden, gate pitch, h0, lengths, candidate), the last three as the C entry points take them."""
+    index = _lib.require_f32(gates, "gates")
     if gates.dim() != 3 or gates.shape[2] % 2:
         raise ValueError("gates must be [seq, batch, 2 * hidden]")
-    dev, (seq, batch, cols) = gates.device, gates.shape
+    seq, batch, cols = gates.shape
+    hidden = cols // 2
     if candidate not in CANDIDATES:
         raise ValueError(f"candidate must be one of {sorted(CANDIDATES)} (got {candidate!r})")
-    if lengths is not None and (lengths.dtype is not torch.int32 or lengths.shape != (batch,) or
-                                lengths.device != dev or not lengths.is_contiguous()):
-        raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on {dev}")
-    return (dev, seq, batch, cols // 2, _step_rows(gates, "gates", gates.shape, dev),
-            _state(h0, "h0", (batch, cols // 2), dev), lengths.data_ptr() if lengths is not None else None,
-            CANDIDATES[candidate])
+    if lengths is not None:
+        import torch
+        if lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.get_device() != index or \
+                not lengths.is_contiguous():
+            raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on cuda:{index}")
+        lengths = lengths.data_ptr()
+    return (index, seq, batch, hidden, cols if gates.is_contiguous() else _step_rows(gates, "gates", gates.shape, index),
+            _state(h0, "h0", batch, hidden, index) if h0 is not None else None, lengths, CANDIDATES[candidate])
 
 
 def gated_scan(gates, h0=None, *, lengths=None, reverse: bool = False, candidate: str = "tanh", out=None, h_n=None,
@@ -274,15 +271,18 @@ def gated_scan(gates, h0=None, *, lengths=None, reverse: bool = False, candidate
     batch, hidden] may have a pitch; h_n [batch, hidden] may be h0 itself.
     Runs asynchronously on `stream` (default: torch's current stream).
     """
-    dev, seq, batch, hidden, ld, h0p, lenp, cand = _scan_args(gates, h0, lengths, candidate)
+    index, seq, batch, hidden, ld, h0p, lenp, cand = _scan_args(gates, h0, lengths, candidate)
     if out is None:
         out, ld_out = _lib.empty(gates, (seq, batch, hidden), stream), hidden
     else:
-        ld_out = _step_rows(out, "out", (seq, batch, hidden), dev)
+        ld_out = _step_rows(out, "out", (seq, batch, hidden), index)
     if h_n is None:
         h_n = _lib.empty(gates, (batch, hidden), stream)
-    _lib.call(dev, stream, _lib.load().jst_scan_forward, gates.data_ptr(), ld, seq, batch, hidden, h0p, lenp, int(reverse),
-              cand, out.data_ptr(), ld_out, _state(h_n, "h_n", (batch, hidden), dev))
+        h_np = h_n.data_ptr()
+    else:
+        h_np = _state(h_n, "h_n", batch, hidden, index)
+    _lib.call(index, stream, _lib.load().jst_scan_forward, gates.data_ptr(), ld, seq, batch, hidden, h0p, lenp, reverse,
+              cand, out.data_ptr(), ld_out, h_np)
     return out, h_n
 
 
@@ -293,17 +293,17 @@ def gated_scan_backward(gates, out, dout, h0=None, *, dh_n=None, lengths=None, r
     dL/dh_n (either may be None: zero).  dgates is [seq, batch, 2 * hidden], 0
     behind a sequence's end; dh0 is None when h0 is.
     """
-    dev, seq, batch, hidden, ld, h0p, lenp, cand = _scan_args(gates, h0, lengths, candidate)
-    ld_out = _step_rows(out, "out", (seq, batch, hidden), dev)
-    ld_dout = _step_rows(dout, "dout", (seq, batch, hidden), dev) if dout is not None else hidden
+    index, seq, batch, hidden, ld, h0p, lenp, cand = _scan_args(gates, h0, lengths, candidate)
+    ld_out = _step_rows(out, "out", (seq, batch, hidden), index)
+    ld_dout = _step_rows(dout, "dout", (seq, batch, hidden), index) if dout is not None else hidden
     if dgates is None:
         dgates, ld_dg = _lib.empty(gates, (seq, batch, 2 * hidden), stream), 2 * hidden
     else:
-        ld_dg = _step_rows(dgates, "dgates", (seq, batch, 2 * hidden), dev)
+        ld_dg = _step_rows(dgates, "dgates", (seq, batch, 2 * hidden), index)
     dh0 = _lib.empty(gates, (batch, hidden), stream) if h0 is not None else None
-    _lib.call(dev, stream, _lib.load().jst_scan_backward, gates.data_ptr(), ld, seq, batch, hidden, h0p, lenp, int(reverse),
+    _lib.call(index, stream, _lib.load().jst_scan_backward, gates.data_ptr(), ld, seq, batch, hidden, h0p, lenp, reverse,
               cand, out.data_ptr(), ld_out, dout.data_ptr() if dout is not None else None, ld_dout,
-              _state(dh_n, "dh_n", (batch, hidden), dev), dgates.data_ptr(), ld_dg,
+              _state(dh_n, "dh_n", batch, hidden, index) if dh_n is not None else None, dgates.data_ptr(), ld_dg,
               dh0.data_ptr() if dh0 is not None else None)
     return dgates, dh0
 
