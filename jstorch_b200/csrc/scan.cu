@@ -375,6 +375,23 @@ struct Steps {
     }
 };
 
+// Zeros behind the sequences: the rows of steps [s, end), every stride-th run of K.
+template <bool BWD, int V, int K>
+__device__ __forceinline__ void write_zeros(const Channels<BWD, V>& w, int64_t s, int64_t end, int64_t stride, int seq) {
+    const Rows& r = BWD ? w.dgates : w.out;
+    for (; s < end; s += stride) {
+        char* o = r.at(s);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            if (w.mine && s + i < seq) {
+                store(o + r.lane, all<V>(0.0f));
+                if (BWD) store(o + w.c + r.lane, all<V>(0.0f));
+            }
+            o += r.step;
+        }
+    }
+}
+
 // The warp's index, known to the compiler as the same in all lanes.
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
@@ -446,8 +463,14 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
     const F<V> h_first = w.state(p.h0);
     F<V> carry = BWD ? w.state(p.dh_n) : h_first;
     const int64_t round_steps = (int64_t)C * S * K, my_first = (int64_t)(rank * S + warp) * K;
+    // The rounds that some channel of the tile has steps in; the others, before
+    // and behind, are zeros alone.  The same in all warps and blocks of the cluster.
+    const int some_lo = __reduce_min_sync(0xffffffffu, w.lo < w.hi ? w.lo : p.seq);
+    const int some_hi = __reduce_max_sync(0xffffffffu, w.lo < w.hi ? w.hi : 0);
+    const int64_t begin = some_lo / round_steps * round_steps;
+    const int64_t end = (some_hi + round_steps - 1) / round_steps * round_steps;
     Raw<BWD, V, K> raw;
-    raw.fetch(p, w, h_first, my_first);
+    raw.fetch(p, w, h_first, begin + my_first);
     if (C > 1) {
         if (threadIdx.x == 0) {
             ptx::mbar_init(&arrived[0], 1);
@@ -459,7 +482,7 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
         ptx::cluster_wait();
     }
     uint32_t round = 0;
-    for (int64_t base = 0; base < p.seq; base += round_steps, ++round) {
+    for (int64_t base = begin; base < end; base += round_steps, ++round) {
         const int parity = round & 1;
         const int64_t s0 = base + my_first;
         if (C > 1 && threadIdx.x == 0) ptx::mbar_arrive_expect_tx(&arrived[parity], (uint32_t)(C * 32 * sizeof(Pair<V>)));
@@ -470,7 +493,7 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
             st.fold(mine.A, mine.B);
             warps[parity][warp][lane] = mine;
         }
-        if (base + round_steps < p.seq) raw.fetch(p, w, h_first, s0 + round_steps);
+        if (base + round_steps < end) raw.fetch(p, w, h_first, s0 + round_steps);
         // One barrier a round: a warp writes these places again two rounds on,
         // past the next barrier, which every warp reaches after reading them.
         __syncthreads();
@@ -513,6 +536,8 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
         st.finish(e, p.seq, w, s0);
     }
     if (rank == 0 && warp == 0) w.set_state(BWD ? p.dh0 : p.h_n, carry);
+    write_zeros<BWD, V, K>(w, my_first, begin, round_steps, p.seq);
+    write_zeros<BWD, V, K>(w, std::max(end, begin) + my_first, p.seq, round_steps, p.seq);
     if (C > 1) {
         if (threadIdx.x == 0 && gave_up) atomicOr(p.err, gave_up);
         ptx::cluster_arrive();  // nobody leaves while another could still send to it
@@ -552,6 +577,9 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 //     4 x 4 200), and where the tiles leave SMs empty, clusters that share a
 //     tile's axis: forward 2 blocks fit an SM, backward 1 (4096 x 1 x 4096:
 //     47 / 83 in clusters of 4 / 2, 94 / 122 without).
+//   * Long sequences of different lengths: twice the clusters, as the tiles of the
+//     longest outlast the others (2048 x 16 x 1024 with lengths drawn evenly:
+//     65 / 110, 78 / 132 without; at 1000 x 64 x 256 it costs, 40 / 68 for 37 / 67).
 //   * So few channels that even clusters of 8 blocks leave SMs empty: one
 //     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 188 / 312
 //     against 240 / 428 with two).
@@ -567,10 +595,11 @@ int run_scan(const ScanArgs& p, cudaStream_t s) {
         return JST_OK;
     }
     if (p.seq <= 64 && tiles >= 4 * sms) return launch_tiled<BWD, TANH, V, 4, 4, BWD ? 5 : 8>(p, 1, s);
-    if (BWD && V == 2 && tiles >= sms) return launch_tiled<BWD, TANH, V, 4, 8, 1>(p, 1, s);
+    const bool uneven = p.lengths && p.seq > 1024;
+    if (BWD && V == 2 && tiles >= sms && !uneven) return launch_tiled<BWD, TANH, V, 4, 8, 1>(p, 1, s);
     constexpr int blocks_per_sm = BWD && V == 2 ? 1 : 2;
     int C = 1;
-    while (C < 8 && tiles * C * 2 <= sms * blocks_per_sm && p.seq > C * 64) C *= 2;
+    while (C < 8 && tiles * C * 2 <= sms * blocks_per_sm * (uneven ? 2 : 1) && p.seq > C * 64) C *= 2;
     return launch_tiled<BWD, TANH, V, 8, 8, blocks_per_sm>(p, C, s);
 }
 
