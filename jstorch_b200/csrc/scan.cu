@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/jstorch_scan.h"
 #include "gemm_internal.h"
@@ -451,10 +452,12 @@ __device__ __forceinline__ void send(Pair<V>* to, uint64_t* bar, int rank, const
                      : "memory");
 }
 
+constexpr int kMostBlocks = 16;  // of a cluster
+
 template <bool BWD, bool TANH, int V, int S, int K, int BLOCKS>
 __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanArgs p, int C) {
     __shared__ Pair<V> warps[2][S][32];   // the warps' folds, two rounds
-    __shared__ Pair<V> blocks[2][8][32];  // the folds of the cluster's blocks, two rounds
+    __shared__ Pair<V> blocks[2][kMostBlocks][32];  // the folds of the cluster's blocks, two rounds
     __shared__ uint64_t arrived[2];
     __shared__ uint32_t gave_up;
     const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -558,6 +561,19 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (C > 8) {  // more than every GPU of the architecture guarantees
+        static bool attr_set[64] = {};
+        static std::mutex mu;
+        int dev = 0;
+        cudaGetDevice(&dev);
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+            if (cudaFuncSetAttribute(scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>,
+                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+                return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(scan_tiled_kernel) failed");
+            attr_set[dev] = true;
+        }
+    }
     ProfScope prof(s, KID_SCAN);
     return cudaLaunchKernelEx(&cfg, scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>, p, C) == cudaSuccess
                ? JST_OK
@@ -582,7 +598,9 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 //     65 / 110, 78 / 132 without; at 1000 x 64 x 256 it costs, 40 / 68 for 37 / 67).
 //   * So few channels that even clusters of 8 blocks leave SMs empty: one
 //     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 188 / 312
-//     against 240 / 428 with two).
+//     against 240 / 428 with two), and where even those leave half the SMs empty,
+//     clusters of 16 (20000 x 1 x 32, identity: 24.8 / 32.1 for 41.0 / 56.3; with
+//     32 tiles they cost, 270 for 190, as fewer such clusters find room).
 template <bool BWD, bool TANH, int V>
 int run_scan(const ScanArgs& p, cudaStream_t s) {
     const int64_t channels = (int64_t)p.batch * p.hidden, tiles = (channels + 32 * V - 1) / (32 * V);
@@ -600,6 +618,7 @@ int run_scan(const ScanArgs& p, cudaStream_t s) {
     constexpr int blocks_per_sm = BWD && V == 2 ? 1 : 2;
     int C = 1;
     while (C < 8 && tiles * C * 2 <= sms * blocks_per_sm * (uneven ? 2 : 1) && p.seq > C * 64) C *= 2;
+    if (C == 8 && tiles * 16 <= sms && p.seq > 8 * 64) C = 16;
     return launch_tiled<BWD, TANH, V, 8, 8, blocks_per_sm>(p, C, s);
 }
 
