@@ -44,7 +44,8 @@ def _aligned(x):
     return held[:, :cols]
 
 
-SIZES = [(1, 1, 1), (1, 7, 3), (1, 128, 64), (1, 1000, 4096), (2, 33, 100), (3, 64, 16), (4, 129, 515), (5, 256, 512),
+SIZES = [(1, 1, 1), (1, 7, 3), (1, 128, 64), (1, 1000, 4096), (1, 20, 1024), (1, 21, 1025), (1, 40, 8192), (1, 33, 8195),
+         (1, 50, 20001), (2, 1, 5), (6, 3000, 700), (16, 5, 640), (40, 130, 2050), (64, 1500, 129), (65, 300, 40), (2, 33, 100), (3, 64, 16), (4, 129, 515), (5, 256, 512),
          (7, 31, 77), (8, 512, 1024), (9, 100, 260), (15, 65, 48), (16, 130, 1000), (17, 64, 128), (31, 200, 96),
          (33, 257, 129), (64, 64, 64), (100, 300, 1031), (127, 128, 127), (128, 256, 128), (129, 257, 144),
          (200, 513, 2000), (256, 1024, 784), (300, 70, 6000), (513, 129, 17), (1000, 5, 300)]
@@ -59,6 +60,44 @@ def test_product(M, N, K, aligned):
     _held(quant.gemm_i8(lay(a), lay(w), _dev(sa), _dev(sw)), oracle.gemm_i8_f64(a, w, sa, sw))
     _held(quant.gemm_i8(lay(a), lay(w), _dev(sa), _dev(sw), bias=_dev(b), relu=True),
           oracle.gemm_i8_f64(a, w, sa, sw, b, True))
+
+
+@pytest.mark.parametrize("M,N,K", [(600, 9000, 300), (2400, 2600, 1000), (4000, 4100, 200), (700, 4096, 128)])
+def test_many_tiles(M, N, K):
+    """Several tiles a processor, in each of the kernel's tile forms; C with and without 16-byte rows."""
+    import torch
+    from jstorch_b200 import quant
+    a, w, sa, sw, b = _operands(M, N, K)
+    want = torch.from_numpy(a).cuda().double() @ torch.from_numpy(w).cuda().double().t()
+    scale = _dev(sa).double()[:, None] * _dev(sw).double()
+    # oracle.gemm_i8_f64 on the device: three roundings of the product, one of the sum
+    value = want * scale + _dev(b).double()
+    bound = 2.0 ** -24 * (3.001 * (want * scale).abs() + value.abs()) * 1.001 + (want.abs() + 1) * 2.0 ** -150
+    for gap in (0, 1):
+        held = torch.full((M, N + gap), 7.0, device="cuda")
+        quant.gemm_i8(_aligned(a), _aligned(w), _dev(sa), _dev(sw), out=held[:, :N], bias=_dev(b))
+        assert bool(((held[:, :N].double() - value).abs() <= bound).all())
+        assert bool((held[:, N:] == 7).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(70000, 33000, 16), (300000, 16, 8192), (1, 300000, 8192)])
+def test_offsets_past_32_bits(M, N, K):
+    """Outputs of more than 2^31 values, operands of more than 2^31 bytes: the last rows and columns are right."""
+    import torch
+    from jstorch_b200 import quant
+    g = torch.Generator(device="cuda").manual_seed(M)
+    a, w = (torch.randint(-128, 128, (n, K), generator=g, device="cuda", dtype=torch.int8) for n in (M, N))
+    sa, sw = (torch.rand(n, generator=g, device="cuda") + 0.5 for n in (M, N))
+    y = quant.gemm_i8(a, w, sa, sw)
+    m, n = min(M, 40), min(N, 40)
+    want = oracle.gemm_i8_f64(a[-m:].cpu().numpy(), w[-n:].cpu().numpy(), sa[-m:].cpu().numpy(), sw[-n:].cpu().numpy())
+    _held(y[-m:, -n:], want)
+    del y, a
+    if M > 1000 and K > 1000:
+        x = torch.randn((M, K), generator=g, device="cuda")
+        q, s = quant.quantize_rows(x)
+        want_q, want_s = oracle.quantize_rows(x[-5:].cpu().numpy())
+        assert np.array_equal(q[-5:].cpu().numpy(), want_q) and np.array_equal(s[-5:].cpu().numpy(), want_s)
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 5, 131071), (9, 70, 131071), (130, 130, 131071)])
@@ -217,6 +256,53 @@ def test_another_stream_and_captured_graphs():
         for (g, held, y), ref in zip(graphs, want):
             assert torch.equal(y, ref)
             held.zero_()
+
+
+def test_threads_on_their_own_streams():
+    """Several host threads at once: the entry points keep nothing of one call for another."""
+    import threading
+
+    import torch
+    from jstorch_b200 import quant
+    sizes = [(1, 300, 500), (6, 64, 1000), (100, 270, 515), (1000, 1000, 512)]
+    cases, want = [], []
+    for M, N, K in sizes:
+        x = np.random.default_rng(M).standard_normal((M, K)).astype(np.float32)
+        _, w, _, sw, _ = _operands(M, N, K)
+        cases.append((_dev(x), _dev(w), _dev(sw)))
+        want.append(quant.linear_i8(*cases[-1]))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for k in range(20):
+                c = (i + k) % len(cases)
+                y = quant.linear_i8(*cases[c])
+                s.synchronize()
+                if not torch.equal(y, want[c]):
+                    bad.append((i, c))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_repeats_bit_for_bit_and_keeps_its_inputs():
+    import torch
+    from jstorch_b200 import quant
+    for M, N, K in ((5, 300, 515), (700, 700, 700)):
+        a, w, sa, sw, b = _operands(M, N, K)
+        held = [_dev(v) for v in (a, w, sa, sw, b)]
+        first = quant.gemm_i8(*held[:4], bias=held[4])
+        assert torch.equal(first, quant.gemm_i8(*held[:4], bias=held[4]))
+        assert all(np.array_equal(h.cpu().numpy(), v) for h, v in zip(held, (a, w, sa, sw, b)))
+    import jstorch_b200
+    assert jstorch_b200.device_error() == 0
 
 
 def test_refusals():
