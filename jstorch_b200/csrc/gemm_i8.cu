@@ -468,19 +468,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 }
 
 // ------------------------------------------------------------ few tokens
-template <int T_, int STAGES_>
+// FP32: the tokens come as fp32 rows.  Every CTA finds their scales and
+// quantises its own part of K into shared memory while its weight is on the way.
+template <int T_, int STAGES_, bool FP32_ = false>
 struct TokCfg {
     static constexpr int T = T_;  // tokens, padded
     static constexpr int STAGES = STAGES_;
+    static constexpr bool FP32 = FP32_;
+    static constexpr int SLABS = 16;  // FP32: k-slabs of a CTA at most
     static constexpr uint32_t TMEM_COLS = T_ < 32 ? 32 : T_;
     static constexpr uint32_t R_BYTES = BM * BK;
     static constexpr uint32_t S_BYTES = T_ * BK;
-    static constexpr uint32_t STAGE_BYTES = R_BYTES + S_BYTES;
-    static constexpr uint32_t EX_OFF = STAGES_ * STAGE_BYTES;  // int32 [cluster][128][tokens of this CTA]
+    static constexpr uint32_t STAGE_BYTES = R_BYTES + (FP32_ ? 0 : S_BYTES);
+    static constexpr uint32_t X_OFF = STAGES_ * STAGE_BYTES;  // FP32: [SLABS] tiles of the tokens
+    static constexpr uint32_t EX_OFF = X_OFF + (FP32_ ? SLABS * S_BYTES : 0);  // int32 [cluster][128][tokens of this CTA]
     static constexpr uint32_t SCALE_OFF = EX_OFF + T_ * BM * 4;
     static constexpr uint32_t BAR_OFF = SCALE_OFF + 256;
     static constexpr uint32_t SMEM_BYTES = BAR_OFF + 256 + 768 /*from 256- to 1024-byte alignment*/;
-    static_assert(SMEM_BYTES <= 227 * 1024 && S_BYTES % 1024 == 0 && (2 * STAGES_ + 1) * 8 + 8 <= 256, "shared memory");
+    static_assert(SMEM_BYTES <= 227 * 1024 && S_BYTES % 1024 == 0 && (2 * STAGES_ + 2) * 8 + 8 <= 256, "shared memory");
 };
 constexpr int TOK_THREADS = 192;
 
@@ -494,7 +499,65 @@ struct TokParams {
     const float* bias;
     int relu;
     uint32_t* err;
+    const float* x;  // FP32: the tokens
+    int64_t ldx;
 };
+
+// FP32: warp w of four takes tokens w, w + 4, ...: the scale of the whole row,
+// then the row's part of K as the swizzled tiles that TMA would have written
+// (16-byte piece j of a 128-byte row r at j ^ (r & 7)), zeros behind M and K.
+template <class C>
+__device__ __forceinline__ void quantize_tokens(const TokParams& p, uint8_t* smem, float* token_scale, uint64_t* x_bar,
+                                                int kb0, int num_kb, int own0, int own, int w, int lane) {
+    constexpr int ROWS = C::T / 4;  // of a warp, side by side: their loads are in flight together
+    const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && (p.tokens == 1 || (p.ldx & 3) == 0);
+    auto fetch = [&](int m, int k) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float* at = p.x + (int64_t)m * p.ldx + k;
+        if (m >= p.tokens) return v;
+        if (vec && k + 4 <= p.K) return __ldg(reinterpret_cast<const float4*>(at));
+        if (k < p.K) v.x = __ldg(at);
+        if (k + 1 < p.K) v.y = __ldg(at + 1);
+        if (k + 2 < p.K) v.z = __ldg(at + 2);
+        if (k + 3 < p.K) v.w = __ldg(at + 3);
+        return v;
+    };
+    uint32_t peak[ROWS] = {};
+#pragma unroll 2
+    for (int k = 4 * lane; k < p.K; k += 128) {
+        float4 v[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) v[i] = fetch(w + 4 * i, k);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+            peak[i] = max(max(max(peak[i], abs_bits(v[i].x)), max(abs_bits(v[i].y), abs_bits(v[i].z))), abs_bits(v[i].w));
+    }
+    float s[ROWS], inv[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int m = w + 4 * i;
+        s[i] = row_scale(__reduce_max_sync(0xffffffffu, peak[i]));
+        inv[i] = row_inverse(s[i]);
+        if (lane == 0 && m >= own0 && m < own0 + own) token_scale[m - own0] = s[i];
+    }
+#pragma unroll 2
+    for (int kb = 0; kb < num_kb; ++kb) {
+        float4 v[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) v[i] = fetch(w + 4 * i, (kb0 + kb) * BK + 4 * lane);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int m = w + 4 * i;
+            uint8_t* tile = smem + C::X_OFF + kb * C::S_BYTES + m * BK;
+            *reinterpret_cast<char4*>(tile + (((lane >> 2) ^ (m & 7)) << 4) + ((lane & 3) << 2)) =
+                make_char4((signed char)quantize_in(v[i].x, s[i], inv[i]), (signed char)quantize_in(v[i].y, s[i], inv[i]),
+                           (signed char)quantize_in(v[i].z, s[i], inv[i]), (signed char)quantize_in(v[i].w, s[i], inv[i]));
+        }
+    }
+    ptx::fence_proxy_async_smem();  // the tensor cores read what these stores wrote
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(x_bar);
+}
 
 //   warp 0      TMA producer (and, before it may read what the launch before
 //               this one wrote, prefetches of its weight slabs into L2)
@@ -511,7 +574,8 @@ __global__ void __launch_bounds__(TOK_THREADS)
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
     uint64_t* empty_bar = full_bar + STAGES;
     uint64_t* accum_bar = empty_bar + STAGES;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum_bar + 1);
+    uint64_t* x_bar = accum_bar + 1;  // FP32: the tokens are quantised
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_bar + 1);
     volatile uint32_t* err = tmem_slot + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -529,10 +593,11 @@ __global__ void __launch_bounds__(TOK_THREADS)
             ptx::mbar_init(&empty_bar[s], 1);
         }
         ptx::mbar_init(accum_bar, 1);
+        ptx::mbar_init(x_bar, 4);  // one arrival per quantising warp
         *err = 0;
         ptx::fence_barrier_init();
         ptx::tma_prefetch_desc(&tm_w);
-        ptx::tma_prefetch_desc(&tm_x);
+        if (!C::FP32) ptx::tma_prefetch_desc(&tm_x);
         for (int kb = 0; kb < num_kb; ++kb) ptx::tma_prefetch_3d(&tm_w, (kb0 + kb) * BK, n0, 0);
     }
     if (warp == 1) ptx::tmem_alloc<C::TMEM_COLS>(tmem_slot);
@@ -542,7 +607,7 @@ __global__ void __launch_bounds__(TOK_THREADS)
     const uint32_t tmem_base = *tmem_slot;
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    if (threadIdx.x < own) token_scale[threadIdx.x] = own0 + threadIdx.x < p.tokens ? __ldg(p.token_scale + own0 + threadIdx.x) : 0.0f;
+    if (!C::FP32 && threadIdx.x < own) token_scale[threadIdx.x] = own0 + threadIdx.x < p.tokens ? __ldg(p.token_scale + own0 + threadIdx.x) : 0.0f;
     if (cluster > 1) {  // nobody writes another's shared memory before that one runs
         ptx::cluster_arrive();
         ptx::cluster_wait();
@@ -556,22 +621,24 @@ __global__ void __launch_bounds__(TOK_THREADS)
                 uint8_t* st = smem + s * C::STAGE_BYTES;
                 ptx::mbar_arrive_expect_tx(&full_bar[s], C::STAGE_BYTES);
                 ptx::tma_load_3d(st, &tm_w, &full_bar[s], (kb0 + kb) * BK, n0, 0);
-                ptx::tma_load_3d(st + C::R_BYTES, &tm_x, &full_bar[s], (kb0 + kb) * BK, 0, 0);
+                if (!C::FP32) ptx::tma_load_3d(st + C::R_BYTES, &tm_x, &full_bar[s], (kb0 + kb) * BK, 0, 0);
             }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = ptx::idesc_i8(BM, C::T);
-            for (int kb = 0; kb < num_kb; ++kb) {
+            const bool ready = !C::FP32 || ptx::mbar_wait(x_bar, 0, err);
+            for (int kb = 0; kb < num_kb && ready; ++kb) {
                 const int s = kb % STAGES;
                 if (!ptx::mbar_wait(&full_bar[s], (kb / STAGES) & 1, err)) break;
                 ptx::tc_fence_after();
                 const uint32_t st = ptx::smem_u32(smem + s * C::STAGE_BYTES);
+                const uint32_t xt = C::FP32 ? ptx::smem_u32(smem + C::X_OFF + kb * C::S_BYTES) : st + C::R_BYTES;
 #pragma unroll
                 for (int kk = 0; kk < BK / 32; ++kk)
                     ptx::mma_i8(tmem_base, ptx::smem_desc_kmajor(st + kk * 32, 128),
-                                ptx::smem_desc_kmajor(st + C::R_BYTES + kk * 32, 128), idesc, (kb | kk) != 0);
+                                ptx::smem_desc_kmajor(xt + kk * 32, 128), idesc, (kb | kk) != 0);
                 ptx::mma_commit(&empty_bar[s]);
             }
             ptx::mma_commit(accum_bar);  // always signalled, also on the error path
@@ -579,6 +646,7 @@ __global__ void __launch_bounds__(TOK_THREADS)
         }
         __syncwarp();
     } else {
+        if (C::FP32) quantize_tokens<C>(p, smem, token_scale, x_bar, kb0, num_kb, own0, own, warp - 2, lane);
         int okw = 0;
         if (lane == 0) okw = ptx::mbar_wait(accum_bar, 0, err) && *err == 0;
         const bool ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
@@ -776,11 +844,13 @@ static bool make_operand_map(CUtensorMap* m, const int8_t* x, int rows, int K, i
     return make_map(m, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, rows, rows == 1 ? ((int64_t)K + 15) / 16 * 16 : ld, box_rows);
 }
 
-static int run_tokens(const I8Args& a, cudaStream_t s) {
+// x: the tokens in fp32 (gemm_i8_tc_takes_fp32), or null.
+static int run_tokens(const I8Args& a, const float* x, int64_t ldx, cudaStream_t s) {
     const int T = a.M <= 16 ? 16 : a.M <= 32 ? 32 : 64;
-    CUtensorMap w, x;
-    if (!make_operand_map(&w, a.B, a.N, a.K, a.ldb, BM) || !make_operand_map(&x, a.A, a.M, a.K, a.lda, T))
-        return set_status(JST_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    CUtensorMap w, xm;
+    if (!make_operand_map(&w, a.B, a.N, a.K, a.ldb, BM)) return set_status(JST_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    xm = w;  // not read with fp32 tokens
+    if (!x && !make_operand_map(&xm, a.A, a.M, a.K, a.lda, T)) return set_status(JST_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     TokParams p{};
     p.channels = a.N; p.tokens = a.M; p.K = a.K;
     p.C = a.C; p.ldc = a.ldc;
@@ -797,13 +867,16 @@ static int run_tokens(const I8Args& a, cudaStream_t s) {
     while (lg < 3 && (8 << lg) <= T && (tiles << (lg + 1)) <= room && (2 << lg) <= slabs) ++lg;
     p.cluster_log2 = lg;
     p.kb_per_rank = (slabs + (1 << lg) - 1) >> lg;
-    if (T == 16) return launch_tokens<TokCfg<16, 5>>(w, x, p, s);
-    if (T == 32) return launch_tokens<TokCfg<32, 4>>(w, x, p, s);
-    return launch_tokens<TokCfg<64, 7>>(w, x, p, s);
+    p.x = x;
+    p.ldx = ldx;
+    if (x) return launch_tokens<TokCfg<16, 4, true>>(w, xm, p, s);
+    if (T == 16) return launch_tokens<TokCfg<16, 5>>(w, xm, p, s);
+    if (T == 32) return launch_tokens<TokCfg<32, 4>>(w, xm, p, s);
+    return launch_tokens<TokCfg<64, 7>>(w, xm, p, s);
 }
 
 static int run_aligned(const I8Args& a, cudaStream_t s) {
-    if (a.M <= 64) return run_tokens(a, s);
+    if (a.M <= 64) return run_tokens(a, nullptr, 0, s);
     // The tile by what it is expected to take, in ns measured on a B200: a k-slab
     // (8192^3: 384 us in pairs, 602 and 1055 in tiles of 128 and 64 columns) or,
     // where K is short, the epilogue (8192 x 8192 x 512: 93, 66, 93) of a tile,
@@ -845,6 +918,19 @@ static int run_aligned(const I8Args& a, cudaStream_t s) {
 }
 
 }  // namespace i8
+
+// Up to 16 tokens of so few values that one launch beats two: such calls wait
+// for the host, which spends 5.1 us on this one and 7.8 on a quantisation, its
+// workspace and the product (5 x 2048 x 512; on the device alone 6.7 and 5.6,
+// and 16 x 1024 x 1024, 10.6 and 6.3).  The weight needs no copy.
+bool gemm_i8_tc_takes_fp32(const I8Args& a) {
+    return a.M <= 16 && (int64_t)a.M * a.K <= 4096 && a.K <= i8::TokCfg<16, 4, true>::SLABS * i8::BK &&
+           i8::aligned(a.B, a.ldb, a.N);
+}
+
+int gemm_i8_tc_run_fp32(const I8Args& a, const float* x, int64_t ldx, cudaStream_t s) {
+    return i8::run_tokens(a, x, ldx, s);
+}
 
 int gemm_i8_tc_run(const I8Args& args, cudaStream_t s) {
     I8Args a = args;

@@ -14,31 +14,6 @@
 namespace jst {
 namespace {
 
-// q = x / s to the nearest integer, ties to even, where s = max|x| * (1 / 127) > 0.
-// x * (1 / s) is within a few 2^-24 of the quotient, so only a value within
-// 2^-12 of a half can round to another integer than the quotient does; those
-// (one in two thousand) divide in 64 bits, which separates every quotient of
-// two fp32 numbers from a half that it does not equal.
-__device__ __forceinline__ int quantize(float x, float s, float inv) {
-    const float t = x * inv;
-    float q = rintf(t);
-    if (!(fabsf(fabsf(t - q) - 0.5f) > 0.000244140625f)) q = (float)rint((double)x / (double)s);
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
-
-// Largest |x| of a row as its bits: the order of non-negative floats is the
-// order of their bits, and a NaN's are above infinity's, so one integer
-// maximum finds the peak and tells a row that is not finite.
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-__device__ __forceinline__ float row_scale(uint32_t peak) {
-    return peak < 0x7f800000u ? __fmul_rn(__uint_as_float(peak), 1.0f / 127.0f) : __uint_as_float(0x7fffffffu);
-}
-// 1 / s, or 0 where the row quantises to zeros (s is 0 or NaN).
-__device__ __forceinline__ float row_inverse(float s) { return s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f; }
-
-__device__ __forceinline__ int quantize_in(float x, float s, float inv) { return inv > 0.0f ? quantize(x, s, inv) : 0; }
-
 // One block a row.  NV > 0: the row's values stay in registers, NV groups of
 // four a thread, between the peak and the quantisation, so x is read once;
 // NV == 0 (rows of more than 32768 values) reads it twice.  Bound by memory: 5
@@ -379,6 +354,10 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
              (epilogue & JST_EPI_RELU) ? 1 : 0, y, ldy};
     if (K == 0 || (M == 1 && K <= kSegment)) {
         rc = K == 0 ? run_empty(p, s) : run_one(p, x, s);
+        return rc ? rc : launched("linear_i8 launch failed");
+    }
+    if (M > 1 && gemm_i8_tc_takes_fp32(p)) {
+        rc = gemm_i8_tc_run_fp32(p, x, ldx, s);
         return rc ? rc : launched("linear_i8 launch failed");
     }
     const int64_t ldq = ((int64_t)K + 15) / 16 * 16;

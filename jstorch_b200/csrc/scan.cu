@@ -587,7 +587,7 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 //     over warps 5.7 / 8.8; 16 x 64 x 1024: 6.2 / 8.0, split 6.1 / 10.1;
 //     128 x 256 x 1024: 71 / 136, split 84 / 150).
 //   * Many tiles of a short axis: small blocks, of which many fit an SM
-//     (64 x 64 x 1024: 11.9 / 18.3; in blocks of 8 warps x 8 steps 15.1 / 24.8).
+//     (64 x 64 x 1024: 12.5 / 19.2; in blocks of 8 warps x 8 steps 15.1 / 24.8).
 //   * Otherwise 64 steps a block and round, 8 a lane (2048 x 16 x 1024 forward
 //     81, with 4 steps a lane 100; backward 4 warps x 8 steps 143, 8 x 8 146,
 //     4 x 4 200), and where the tiles leave SMs empty, clusters that share a
@@ -612,7 +612,7 @@ int run_scan(const ScanArgs& p, cudaStream_t s) {
         scan_serial_kernel<BWD, TANH, V, 4><<<(unsigned)grid, kSerialThreads, 0, s>>>(p);
         return JST_OK;
     }
-    if (p.seq <= 64 && tiles >= 4 * sms) return launch_tiled<BWD, TANH, V, 4, 4, BWD ? 5 : 8>(p, 1, s);
+    if (p.seq <= 64 && tiles >= 4 * sms) return launch_tiled<BWD, TANH, V, 4, 4, BWD ? 5 : 7>(p, 1, s);
     const bool uneven = p.lengths && p.seq > 1024;
     if (BWD && V == 2 && tiles >= sms && !uneven) return launch_tiled<BWD, TANH, V, 4, 8, 1>(p, 1, s);
     constexpr int blocks_per_sm = BWD && V == 2 ? 1 : 2;

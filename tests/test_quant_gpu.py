@@ -199,7 +199,9 @@ def test_linear(M, N, K):
     assert np.array_equal(y.cpu().numpy(), quant.gemm_i8(qd, _aligned(w), sd, _dev(sw), bias=_dev(b)).cpu().numpy())
     # rows with a pitch, a weight without alignment
     held = _dev(np.concatenate([x, x[:, :1] + 9], axis=1))
-    _held(quant.linear_i8(held[:, :K], _dev(w), _dev(sw), bias=_dev(b), relu=True), oracle.gemm_i8_f64(q, w, s, sw, b, True))
+    want = oracle.gemm_i8_f64(q, w, s, sw, b, True)
+    _held(quant.linear_i8(held[:, :K], _dev(w), _dev(sw), bias=_dev(b), relu=True), want)
+    _held(quant.linear_i8(held[:, :K], _aligned(w), _dev(sw), bias=_dev(b), relu=True), want)
 
 
 @pytest.mark.parametrize("repeat", [1, 20])
