@@ -58,7 +58,7 @@ __device__ __forceinline__ float drop(float v, uint32_t word, const DropoutArgs&
 
 // One row, or rows without gaps: group g holds elements 4g .. 4g + 3.  A thread
 // has the loads of G groups in flight while it makes their words: 67108864
-// elements take 105 us with one, 91 with two, 85.5 with four (6.3 TB/s, 0.96 of
+// elements take 105 us with one, 91 with two, 80.4 with four (6.7 TB/s, 1.02 of
 // the measured copy rate); 65536 elements, 1.5 us with one, 2.0 with four, as
 // fewer SMs have work.
 // VEC: both buffers are 16-byte aligned.
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) dropout_flat_kernel(const DropoutArg
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 const int64_t g = g0 + i * kThreads;
-                if (g < whole) v[i] = __ldcs(reinterpret_cast<const float4*>(a.x) + g);
+                if (g < whole) v[i] = reinterpret_cast<const float4*>(a.x)[g];
             }
 #pragma unroll
         for (int i = 0; i < G; ++i) {

@@ -19,8 +19,9 @@ namespace {
 // NV == 0 (rows of more than 32768 values) reads it twice.  Bound by memory: 5
 // bytes a value.  VEC: x and q rows allow 16- and 4-byte accesses.
 template <int NV, bool VEC>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const float* __restrict__ x, int64_t ldx, int cols, int8_t* __restrict__ q,
-                                     int64_t ldq, float* __restrict__ scale) {
+__global__ void __launch_bounds__(1024)
+    quantize_rows_kernel(const float* __restrict__ x, int64_t ldx, int cols, int8_t* __restrict__ q, int64_t ldq,
+                         float* __restrict__ scale) {
     __shared__ uint32_t part[32];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
@@ -28,7 +29,7 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const float* __rest
     int8_t* out = q + (int64_t)blockIdx.x * ldq;
     const int n = blockDim.x;
     auto fetch = [&](int k) {
-        if (VEC && k + 4 <= cols) return __ldcs(reinterpret_cast<const float4*>(row + k));
+        if (VEC && k + 4 <= cols) return __ldg(reinterpret_cast<const float4*>(row + k));
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (k < cols) v.x = row[k];
         if (k + 1 < cols) v.y = row[k + 1];
