@@ -549,9 +549,7 @@ __device__ __forceinline__ void quantize_tokens(const TokParams& p, uint8_t* sme
         for (int i = 0; i < ROWS; ++i) {
             const int m = w + 4 * i;
             uint8_t* tile = smem + C::X_OFF + kb * C::S_BYTES + m * BK;
-            *reinterpret_cast<char4*>(tile + (((lane >> 2) ^ (m & 7)) << 4) + ((lane & 3) << 2)) =
-                make_char4((signed char)quantize_in(v[i].x, s[i], inv[i]), (signed char)quantize_in(v[i].y, s[i], inv[i]),
-                           (signed char)quantize_in(v[i].z, s[i], inv[i]), (signed char)quantize_in(v[i].w, s[i], inv[i]));
+            *reinterpret_cast<uint32_t*>(tile + (((lane >> 2) ^ (m & 7)) << 4) + ((lane & 3) << 2)) = quantize4(v[i], s[i], inv[i]);
         }
     }
     ptx::fence_proxy_async_smem();  // the tensor cores read what these stores wrote

@@ -143,7 +143,8 @@ def test_output_pitch_leaves_gaps_alone(M):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 5), (2, 16), (5, 255), (4, 256), (7, 1000), (2, 4097), (33, 8192),
-                                       (1, 20000), (3, 40001)])
+                                       (1, 20000), (3, 40001), (1200, 1),
+                                       (1500, 100), (1203, 1021), (1184, 1024), (1300, 1025)])
 def test_quantize_rows(rows, cols):
     from jstorch_b200 import quant
     rng = np.random.default_rng([rows, cols])
