@@ -186,6 +186,26 @@ def test_quantize_hard_rows(cols):
     np.testing.assert_array_equal(q.cpu().numpy(), want_q)
 
 
+def test_quantize_borders():
+    """Every half within the range, and the numbers up to three steps around it, at scales of every size."""
+    from jstorch_b200 import quant
+    rng = np.random.default_rng(3)
+    scales = np.exp(rng.uniform(np.log(1e-37), np.log(1e36), 300)).astype(np.float32)
+    scales = np.concatenate([scales, np.float32(2.0) ** np.arange(-104, -96, dtype=np.float32), np.float32([1.0, 0.75])])
+    halves = np.arange(-126.5, 127.0)
+    x = (halves[None, :, None] * scales.astype(np.float64)[:, None, None]).astype(np.float32)
+    x = np.repeat(x, 7, axis=2)
+    for k in range(7):
+        for _ in range(abs(k - 3)):
+            x[..., k] = np.nextafter(x[..., k], np.float32(np.inf if k > 3 else -np.inf))
+    x = x.reshape(len(scales), -1)
+    x[:, 0] = np.float32(127.0) * scales
+    q, s = quant.quantize_rows(_dev(x))
+    want_q, want_s = oracle.quantize_rows(x)
+    np.testing.assert_array_equal(s.cpu().numpy(), want_s)
+    np.testing.assert_array_equal(q.cpu().numpy(), want_q)
+
+
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_linear(M, N, K):
     from jstorch_b200 import quant
