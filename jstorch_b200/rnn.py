@@ -42,7 +42,8 @@ class _TrainContext:
 
 class _LayerDropout:
     """Dropout between stacked layers: layer l of the model's n-th training
-    pass has the mask of (seed, offset n * num_layers + l)."""
+    pass has the mask of (seed, offset n * num_layers + l).  A captured graph
+    repeats the pass that it was captured in, masks included."""
 
     def _init_dropout(self, dropout: float, seed: int) -> None:
         if not 0.0 <= dropout <= 1.0:
