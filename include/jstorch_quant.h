@@ -19,8 +19,9 @@ extern "C" {
  * 0 and q = 0; a row that holds an infinity or a NaN has scale NaN and q = 0, so
  * every product of it is NaN (0 behind a ReLU, as in jst_gemm_ex).
  *   x  row r at x + r * ldx, ldx >= cols;   q  row r at q + r * ldq, ldq >= cols
- * The bytes of a q row behind `cols` are left as they were.  A pitch that is a
- * multiple of 16 (and a 16-byte aligned q) lets jst_gemm_i8 read it in place.
+ * rows and cols are at most 0x7fff0000; the arrays do not overlap.  The bytes of
+ * a q row behind `cols` are left as they were.  A pitch that is a multiple of 16
+ * (and a 16-byte aligned q) lets jst_gemm_i8 read it in place.
  */
 int jst_quantize_rows_i8(const float* x, int64_t ldx, int rows, int cols, int8_t* q, int64_t ldq, float* scale,
                          jst_stream_t stream);
@@ -36,6 +37,7 @@ int jst_quantize_rows_i8(const float* x, int64_t ldx, int rows, int cols, int8_t
  *   epilogue: JST_EPI_NONE, JST_EPI_BIAS, JST_EPI_RELU or JST_EPI_BIAS_RELU.
  *   An operand whose address or pitch is not a multiple of 16 bytes is first
  *   copied to an aligned workspace where the tensor cores compute the product.
+ * M and N are at most 0x7fff0000; C overlaps no operand.
  * K == 0 writes epilogue(0).  Asynchronous on `stream`; repeats bit for bit.
  */
 typedef struct jst_gemm_i8_desc {

@@ -248,13 +248,22 @@ int launched(const char* what) {
     return cudaPeekAtLastError() == cudaSuccess ? set_status(JST_OK, nullptr) : set_status(JST_ERR_CUDA, what);
 }
 
+// Rows and columns up to this: the kernels count in 32 bits and round up to tiles.
+constexpr int kMost = 0x7fff0000;
+
 int check_quantize(const float* x, int64_t ldx, int rows, int cols, const int8_t* q, int64_t ldq, const float* scale) {
     if (rows < 0 || cols < 0) return set_status(JST_ERR_ARG, "quantize_rows: negative size");
+    if (rows > kMost || cols > kMost) return set_status(JST_ERR_ARG, "quantize_rows: size > 0x7fff0000");
     if (rows == 0) return JST_OK;
     if (!scale || (cols > 0 && (!x || !q))) return set_status(JST_ERR_ARG, "quantize_rows: null pointer");
     if (rows > 1 && (ldx < cols || ldq < cols)) return set_status(JST_ERR_ARG, "quantize_rows: pitch < cols");
     if (rows > 1 && (ldx > INT64_MAX / 8 / rows || ldq > INT64_MAX / 8 / rows))
         return set_status(JST_ERR_ARG, "quantize_rows: size exceeds 64 bits");
+    if (cols == 0) return JST_OK;
+    const int64_t span_x = ((rows - 1) * ldx + cols) * 4, span_q = (rows - 1) * ldq + cols, span_s = (int64_t)rows * 4;
+    if (ranges_overlap(q, span_q, x, span_x) || ranges_overlap(scale, span_s, x, span_x) ||
+        ranges_overlap(scale, span_s, q, span_q))
+        return set_status(JST_ERR_ARG, "quantize_rows: an output overlaps another array");
     return JST_OK;
 }
 
@@ -288,6 +297,7 @@ int run_quantize(const float* x, int64_t ldx, int rows, int cols, int8_t* q, int
 int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* b_scale, const float* bias,
                   int epilogue, const float* C, int64_t ldc) {
     if (M < 0 || N < 0 || K < 0) return set_status(JST_ERR_ARG, "gemm_i8: negative size");
+    if (M > kMost || N > kMost) return set_status(JST_ERR_ARG, "gemm_i8: size > 0x7fff0000");
     if (K > 131071) return set_status(JST_ERR_ARG, "gemm_i8: K > 131071 (the sum could exceed 32 bits)");
     if (epilogue < JST_EPI_NONE || epilogue > JST_EPI_BIAS_RELU) return set_status(JST_ERR_ARG, "gemm_i8: unknown epilogue");
     if ((epilogue & JST_EPI_BIAS) && !bias) return set_status(JST_ERR_ARG, "gemm_i8: bias epilogue without a bias pointer");
@@ -296,6 +306,8 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     if ((M > 1 && ldc < N) || (N > 1 && K > 0 && ldb < K)) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
     if ((M > 1 && ldc > INT64_MAX / 8 / M) || (N > 1 && ldb > INT64_MAX / 8 / N))
         return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
+    if (K > 0 && ranges_overlap(C, ((M - 1) * ldc + N) * 4, B, (N - 1) * ldb + K))
+        return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the weight");
     return JST_OK;
 }
 
@@ -326,6 +338,8 @@ extern "C" int jst_gemm_i8(const jst_gemm_i8_desc* d) {
         if (!d->a_scale || (d->K > 0 && !d->A)) return set_status(JST_ERR_ARG, "gemm_i8: null pointer");
         if (d->M > 1 && d->K > 0 && d->lda < d->K) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
         if (d->M > 1 && d->lda > INT64_MAX / 8 / d->M) return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
+        if (d->K > 0 && ranges_overlap(d->C, ((d->M - 1) * d->ldc + d->N) * 4, d->A, (d->M - 1) * d->lda + d->K))
+            return set_status(JST_ERR_ARG, "gemm_i8: C overlaps A");
     }
     rc = require_device();
     if (rc) return rc;
@@ -345,6 +359,8 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
         if (K > 0 && !x) return set_status(JST_ERR_ARG, "linear_i8: null pointer");
         if (M > 1 && ldx < K) return set_status(JST_ERR_ARG, "linear_i8: pitch too small");
         if (M > 1 && ldx > INT64_MAX / 8 / M) return set_status(JST_ERR_ARG, "linear_i8: size exceeds 64 bits");
+        if (K > 0 && ranges_overlap(y, ((M - 1) * ldy + N) * 4, x, ((M - 1) * ldx + K) * 4))
+            return set_status(JST_ERR_ARG, "linear_i8: y overlaps x");
     }
     rc = require_device();
     if (rc) return rc;

@@ -80,6 +80,7 @@ def _desc(**change):
     {"M": -1}, {"N": -1}, {"K": -1}, {"K": 131072, "lda": 131072, "ldb": 131072}, {"lda": 15}, {"ldb": 15}, {"ldc": 4},
     {"A": None}, {"B": None}, {"C": None}, {"a_scale": None}, {"b_scale": None}, {"bias": None, "epilogue": 1},
     {"epilogue": 4}, {"epilogue": 8}, {"epilogue": -1}, {"lda": 1 << 62}, {"ldb": 1 << 62}, {"ldc": 1 << 62},
+    {"M": 0x7fff0001}, {"N": 0x7fff0001, "ldc": 0x7fff0001}, {"C": G + 60}, {"C": OUT + 76},
 ])
 def test_gemm_i8_refusals(bad):
     lib = _lib.load()
@@ -94,6 +95,7 @@ def _linear(x=G, ldx=16, M=4, K=16, w=OUT, ldw=16, ws=HN, N=5, bias=DH0, epilogu
 @pytest.mark.parametrize("bad", [
     {"M": -1}, {"K": 131072, "ldx": 131072, "ldw": 131072}, {"x": None}, {"w": None}, {"ws": None}, {"y": None},
     {"bias": None}, {"epilogue": 5}, {"ldx": 15}, {"ldw": 15}, {"ldy": 4}, {"ldx": 1 << 62},
+    {"M": 0x7fff0001}, {"N": 0x7fff0001, "ldy": 0x7fff0001}, {"y": G + 240}, {"y": OUT + 76},
 ])
 def test_linear_i8_refusals(bad):
     assert _linear(**bad) == 1
@@ -103,7 +105,8 @@ def test_quantize_rows_refusals():
     lib = _lib.load()
     good = dict(x=G, ldx=16, rows=4, cols=16, q=OUT, ldq=16, scale=HN)
     for bad in ({"rows": -1}, {"cols": -1}, {"x": None}, {"q": None}, {"scale": None}, {"ldx": 15}, {"ldq": 15},
-                {"ldx": 1 << 62}, {"ldq": 1 << 62}):
+                {"ldx": 1 << 62}, {"ldq": 1 << 62}, {"q": G + 32}, {"scale": G}, {"scale": OUT + 60},
+                {"rows": 0x7fff0001}, {"rows": 1, "cols": 0x7fff0001}):
         a = {**good, **bad}
         assert lib.jst_quantize_rows_i8(a["x"], a["ldx"], a["rows"], a["cols"], a["q"], a["ldq"], a["scale"], None) == 1
 
