@@ -14,11 +14,11 @@
 //
 // Bytes a step and channel: forward 8 read, 4 written; backward 16 read, 8
 // written; nothing but the outputs is kept for the backward pass, which makes
-// the gates again.  Reached on a B200 (tanh): 2048 x 16 x 1024 forward 81 us
-// (5.0 TB/s, 0.76 of the measured copy rate), backward 143 us (5.6 TB/s, 0.86);
-// 65536 x 1 x 1024, identity, 188 us (4.3 TB/s) and 312 us (5.2 TB/s), where
+// the gates again.  Reached on a B200 (tanh): 2048 x 16 x 1024 forward 79 us
+// (5.1 TB/s, 0.78 of the measured copy rate), backward 138 us (5.8 TB/s, 0.89);
+// 65536 x 1 x 1024, identity, 184 us (4.4 TB/s) and 286 us (5.6 TB/s), where
 // one tile's rounds follow each other.  Forward, what is left is issue slots:
-// 40 instructions for 12 bytes.
+// 38 instructions for 12 bytes.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -599,7 +599,7 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 //   * Many tiles of a short axis: small blocks, of which many fit an SM
 //     (64 x 64 x 1024: 12.5 / 19.2; in blocks of 8 warps x 8 steps 15.1 / 24.8).
 //   * Otherwise 64 steps a block and round, 8 a lane (2048 x 16 x 1024 forward
-//     81, with 4 steps a lane 100; backward 4 warps x 8 steps 143, 8 x 8 146,
+//     79, with 4 steps a lane 100; backward 4 warps x 8 steps 138, 8 x 8 146,
 //     4 x 4 200), and where the tiles leave SMs empty, clusters that share a
 //     tile's axis: forward 2 blocks fit an SM, backward 1 (4096 x 1 x 4096:
 //     47 / 83 in clusters of 4 / 2, 94 / 122 without).
@@ -607,7 +607,7 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 //     longest outlast the others (2048 x 16 x 1024 with lengths drawn evenly:
 //     65 / 110, 78 / 132 without; at 1000 x 64 x 256 it costs, 40 / 68 for 37 / 67).
 //   * So few channels that even clusters of 8 blocks leave SMs empty: one
-//     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 188 / 312
+//     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 184 / 286
 //     against 240 / 428 with two), and where even those leave half the SMs empty,
 //     clusters of 16 (20000 x 1 x 32, identity: 24.8 / 32.1 for 41.0 / 56.3; with
 //     32 tiles they cost, 270 for 190, as fewer such clusters find room).
@@ -659,7 +659,7 @@ int check(const ScanArgs& p, int candidate, bool backward) {
     if (rows == 0 || H == 0) return JST_OK;
     const int64_t most = INT64_MAX / 8 / rows;
     if (p.ld_gates < 2 * H || p.ld_out < H) return set_status(JST_ERR_ARG, "scan: pitch too small");
-    // a warp's channels may lie in 64 rows: their distance is held in 32 bits
+    // a warp's channels may lie in 32 rows: their distance is held in 32 bits
     const int64_t wide = 1 << 24;
     if (p.ld_gates >= wide || p.ld_out >= wide || (backward && (p.ld_dgates >= wide || (p.dout && p.ld_dout >= wide))))
         return set_status(JST_ERR_ARG, "scan: pitch >= 2^24");
