@@ -596,7 +596,8 @@ __global__ void __launch_bounds__(TOK_THREADS)
         ptx::fence_barrier_init();
         ptx::tma_prefetch_desc(&tm_w);
         if (!C::FP32) ptx::tma_prefetch_desc(&tm_x);
-        for (int kb = 0; kb < num_kb; ++kb) ptx::tma_prefetch_3d(&tm_w, (kb0 + kb) * BK, n0, 0);
+        // no more of a long row than fits L2 for all CTAs together
+        for (int kb = 0; kb < min(num_kb, 16); ++kb) ptx::tma_prefetch_3d(&tm_w, (kb0 + kb) * BK, n0, 0);
     }
     if (warp == 1) ptx::tmem_alloc<C::TMEM_COLS>(tmem_slot);
     ptx::tc_fence_before();
