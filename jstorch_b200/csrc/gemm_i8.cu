@@ -931,6 +931,10 @@ int gemm_i8_tc_run_fp32(const I8Args& a, const float* x, int64_t ldx, cudaStream
     return i8::run_tokens(a, x, ldx, s);
 }
 
+bool gemm_i8_tc_in_place(const I8Args& a) {
+    return i8::aligned(a.A, a.lda, a.M) && i8::aligned(a.B, a.ldb, a.N);
+}
+
 int gemm_i8_tc_run(const I8Args& args, cudaStream_t s) {
     I8Args a = args;
     const bool copy_a = !i8::aligned(a.A, a.lda, a.M), copy_b = !i8::aligned(a.B, a.ldb, a.N);

@@ -81,6 +81,8 @@ __device__ __forceinline__ uint32_t quantize4(const float4& x, float s, float in
 
 // The tensor-core kernels (K > 0, M > 0, N > 0).
 int gemm_i8_tc_run(const I8Args& a, cudaStream_t s);
+// Whether gemm_i8_tc_run reads A and B where they are.
+bool gemm_i8_tc_in_place(const I8Args& a);
 // The same with the tokens in fp32 (row pitch ldx), quantised by the product's
 // own blocks: a.A and a.a_scale are unused.  For calls that this takes.
 bool gemm_i8_tc_takes_fp32(const I8Args& a);
