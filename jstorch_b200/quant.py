@@ -19,6 +19,8 @@ def _matrix(x, name: str):
     if x.dim() != 2:
         raise ValueError(f"{name} must be 2-D")
     rows, cols = x.shape
+    if max(rows, cols) > 0x7fff0000:
+        raise ValueError(f"{name}: size > 0x7fff0000")
     if x.is_contiguous():
         return rows, cols, cols or 1
     pitch, unit = x.stride()

@@ -240,6 +240,15 @@ def _state(h, name: str, batch: int, hidden: int, index: int) -> int:
     return h.data_ptr()
 
 
+def _lengths(lengths, batch: int, index: int):
+    """lengths, checked to be a contiguous int32 tensor [batch]."""
+    import torch
+    if lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.get_device() != index or \
+            not lengths.is_contiguous():
+        raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on cuda:{index}")
+    return lengths
+
+
 def _scan_args(gates, h0, lengths, candidate):
     """(device index, seq, batch, hidden, gate pitch, h0, lengths, candidate), the last three as the C entry points take them."""
     index = _lib.require_f32(gates, "gates")
@@ -247,14 +256,12 @@ def _scan_args(gates, h0, lengths, candidate):
         raise ValueError("gates must be [seq, batch, 2 * hidden]")
     seq, batch, cols = gates.shape
     hidden = cols // 2
+    if max(seq, batch, cols) > 0x7fffffff:
+        raise ValueError("gates: size > 2^31 - 1")
     if candidate not in CANDIDATES:
         raise ValueError(f"candidate must be one of {sorted(CANDIDATES)} (got {candidate!r})")
     if lengths is not None:
-        import torch
-        if lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.get_device() != index or \
-                not lengths.is_contiguous():
-            raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on cuda:{index}")
-        lengths = lengths.data_ptr()
+        lengths = _lengths(lengths, batch, index).data_ptr()
     return (index, seq, batch, hidden, cols if gates.is_contiguous() else _step_rows(gates, "gates", gates.shape, index),
             _state(h0, "h0", batch, hidden, index) if h0 is not None else None, lengths, CANDIDATES[candidate])
 
