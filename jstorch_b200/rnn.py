@@ -322,7 +322,8 @@ class GatedRNN(_LayerDropout):
 
     Parameters weight_l{l}[_reverse] [2H, in] and bias_l{l}[_reverse] [2H], rows
     (a | c).  x [seq, batch, in] (or [batch, seq, in] with batch_first), h0
-    [num_layers * directions, batch, H], lengths int32 [batch] as in gated_scan.
+    [num_layers * directions, batch, H], lengths int32 [batch] as in gated_scan:
+    what x and dout hold behind a sequence reaches no result.
     """
 
     def __init__(self, input_size: int, hidden_size: int, num_layers: int = 1, bidirectional: bool = False,
@@ -385,6 +386,9 @@ class GatedRNN(_LayerDropout):
             raise ValueError(f"x must be [seq, batch, {self.input_size}]")
         x = x.contiguous()
         seq, batch, H, dirs = x.shape[0], x.shape[1], self.hidden_size, len(self._suffixes())
+        if train and lengths is not None:  # rows behind a sequence meet dgates of 0 in the weights' gradient
+            behind = torch.arange(seq, device=x.device)[:, None] >= _lengths(lengths, batch, x.get_device())
+            x = x.masked_fill(behind[..., None], 0.0)
         if h0 is not None and (tuple(h0.shape) != (self.num_layers * dirs, batch, H) or not h0.is_contiguous()):
             raise ValueError("h0 must be a contiguous [num_layers * num_directions, batch, hidden]")
         h_n = torch.empty((self.num_layers * dirs, batch, H), dtype=torch.float32, device=x.device)

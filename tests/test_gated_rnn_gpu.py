@@ -86,6 +86,31 @@ def test_training_step(layers, bidir, batch_first, candidate, p):
     assert all(torch.equal(model.grads[k], before[k] + before[k]) for k in before)
 
 
+@pytest.mark.parametrize("batch_first", [False, True])
+def test_padding_does_not_reach_the_gradients(batch_first):
+    """Infinities and NaN behind the sequences, in x and in dout, give the gradients that zeros give."""
+    import torch
+    from jstorch_b200.rnn import GatedRNN
+    model = GatedRNN(9, 11, 2, True, batch_first, dropout=0.25)
+    lengths = torch.tensor([6, 0, 3], dtype=torch.int32, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x, dout = (torch.randn((3, 6, n), generator=gen, device="cuda") for n in (9, 22))
+    behind = (torch.arange(6, device="cuda") >= lengths[:, None])[..., None]
+    results = []
+    for fill in (0.0, float("nan"), float("inf")):
+        model.calls, model.grads = 0, {}
+        a, b = (torch.where(behind, torch.full_like(t, fill), t) for t in (x, dout))
+        if not batch_first:
+            a, b = a.transpose(0, 1), b.transpose(0, 1)
+        given = a.clone()
+        out, h_n, ctx = model.forward_train(a, None, lengths)
+        dx, _ = model.backward(ctx, b)
+        assert torch.equal(a.nan_to_num(), given.nan_to_num())  # x is the caller's
+        results.append([out, h_n, dx, *model.grads.values()])
+    for other in results[1:]:
+        assert all(torch.equal(r, w) for r, w in zip(other, results[0]))
+
+
 def test_gradients_against_differences():
     """dL along a direction of every parameter, against (L(+s) - L(-s)) / 2s in
     fp32: each L rounds to 2e-6 of the sum of its terms' magnitudes, over 2s."""
@@ -192,6 +217,8 @@ def test_refusals():
     x = torch.zeros((3, 2, 4), device="cuda")
     for call in (lambda: model(x[0]), lambda: model(x[..., :3]), lambda: model(x, torch.zeros((1, 2, 6), device="cuda")),
                  lambda: model.step(x[0], torch.zeros((2, 2, 6), device="cuda")),
+                 lambda: model.forward_train(x, None, torch.zeros(3, dtype=torch.int32, device="cuda")),
+                 lambda: model.forward_train(x, None, torch.zeros(2, dtype=torch.int32)),
                  lambda: model.load_state_dict({"bias_l0": torch.zeros(3)}),
                  lambda: GatedRNN(4, 6).step(x[0], torch.zeros((1, 3, 6), device="cuda"))):
         with pytest.raises(ValueError):
