@@ -69,6 +69,7 @@ class GemmI8Desc(ctypes.Structure):
 
 
 _lib = None
+_calls = None
 
 
 def load() -> ctypes.CDLL:
@@ -182,6 +183,18 @@ def launch_count() -> int:
     return int(load().jst_launch_count())
 
 
+def calls():
+    """The extension module _calls (csrc/calls.cpp); raises if it is not built."""
+    global _calls
+    if _calls is None:
+        import torch  # noqa: F401  (the libraries that the extension is linked to)
+
+        load()
+        from . import _calls as module
+        _calls = module
+    return _calls
+
+
 def check(status: int) -> None:
     """Raise JstError for a non-OK status, with the library's message."""
     if status != JST_OK:
@@ -206,38 +219,6 @@ def require_f32(x, name: str) -> int:
     if index < 0 or not x.is_cuda:
         raise ValueError(f"{name} must live on a CUDA device")
     return index
-
-
-def empty(like, shape, stream):
-    """An uninitialised tensor on like's device, of its type, that belongs to
-    `stream`: memory that torch's allocator reuses in another stream's order
-    could still be in use there when `stream` writes it."""
-    if stream is None:
-        return like.new_empty(shape)
-    import torch
-
-    with torch.cuda.stream(stream):
-        return like.new_empty(shape)
-
-
-def call(index: int, stream, function, *args) -> None:
-    """function(*args, stream handle) with device `index` current, on `stream`
-    (by default torch's current stream of the device); raises on a status."""
-    import torch
-
-    if stream is None:
-        handle = torch._C._cuda_getCurrentRawStream(index)  # a Stream object costs 2 us a call
-    elif stream.device.index != index:
-        raise ValueError(f"stream belongs to {stream.device}, the tensors to cuda:{index}")
-    else:
-        handle = stream.cuda_stream
-    if torch._C._cuda_getDevice() == index:
-        status = function(*args, handle)
-    else:
-        with torch.cuda.device(index):
-            status = function(*args, handle)
-    if status:
-        check(status)
 
 
 def header_functions(header: Path = HEADER) -> list[str]:

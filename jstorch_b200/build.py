@@ -7,6 +7,7 @@
 Outputs (git-ignored, shipped with the source tree):
     jstorch_b200/libjstorch_gemm.so   the C-ABI GEMM library (include/jstorch_{gemm,conv,rnn,scan,dropout,quant}.h)
     jstorch_b200/_core*.so            the host core (Tensor / GradTensor), Python extension
+    jstorch_b200/_calls*.so           torch tensors to the scan, dropout and quant entry points
     jstorch_b200/libjstorch_dist.so   the NCCL sharded GEMMs (include/jstorch_dist.h)
 
 Every CUDA source is compiled for sm_100a only
@@ -117,6 +118,31 @@ def build_core(force: bool = False, verbose: bool = False) -> Path:
     return CORE_EXT
 
 
+CALLS_EXT = PKG / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_calls(force: bool = False, verbose: bool = False) -> Path:
+    """_calls: torch tensors to the scan, dropout and quant entry points of
+    libjstorch_gemm.so (found next to it at run time)."""
+    import torch
+
+    BUILD.mkdir(exist_ok=True)
+    root = Path(torch.__file__).parent
+    src, o = CSRC / "calls.cpp", BUILD / "calls.o"
+    headers = [INCLUDE / f"jstorch_{n}.h" for n in ("gemm", "scan", "dropout", "quant")]
+    if force or not _newer(o, [src] + headers + [Path(__file__)]):
+        _run([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", f"-I{CUDA_HOME}/include",
+              f"-I{sysconfig.get_paths()['include']}", "-isystem", str(root / "include"), "-isystem",
+              str(root / "include/torch/csrc/api/include"),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-c", str(src), "-o", str(o)], verbose)
+    if force or not _newer(CALLS_EXT, [o, GEMM_LIB]):
+        tmp = CALLS_EXT.with_suffix(".tmp")
+        _run([CXX, "-shared", "-o", str(tmp), str(o), f"-L{PKG}", "-ljstorch_gemm", f"-L{root / 'lib'}", "-ltorch_python",
+              "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"], verbose)
+        os.replace(tmp, CALLS_EXT)
+    return CALLS_EXT
+
+
 DIST_SOURCES = ["dist.cu", "symm.cu", "reg.cu"]
 DIST_LIB = PKG / "libjstorch_dist.so"
 
@@ -145,6 +171,7 @@ def build_dist(force: bool = False, verbose: bool = False) -> Path:
 def build_all(force: bool = False, ptxas_v: bool = False, verbose: bool = False) -> None:
     build_gemm(force=force, ptxas_v=ptxas_v, verbose=verbose)
     build_core(force=force, verbose=verbose)
+    build_calls(force=force, verbose=verbose)
     build_dist(force=force, verbose=verbose)
 
 
@@ -155,7 +182,7 @@ def main() -> None:
     ap.add_argument("-v", "--verbose", action="store_true")
     a = ap.parse_args()
     build_all(force=a.force, ptxas_v=a.ptxas_v, verbose=a.verbose)
-    print(f"built {GEMM_LIB.relative_to(ROOT)} {CORE_EXT.relative_to(ROOT)} {DIST_LIB.relative_to(ROOT)}")
+    print(f"built {GEMM_LIB.relative_to(ROOT)} {CORE_EXT.relative_to(ROOT)} {CALLS_EXT.relative_to(ROOT)} {DIST_LIB.relative_to(ROOT)}")
 
 
 if __name__ == "__main__":

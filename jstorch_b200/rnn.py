@@ -219,51 +219,10 @@ class GRU(_LayerDropout):
 CANDIDATES = {"tanh": 0, "identity": 1}  # JST_SCAN_* (include/jstorch_scan.h)
 
 
-def _step_rows(x, name: str, shape, index: int) -> int:
-    """Row pitch of a float32 tensor [seq, batch, cols] whose rows are equally far apart."""
-    if _lib.require_f32(x, name) != index or x.shape != shape:
-        raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)} on cuda:{index}")
-    seq, batch, cols = shape
-    if x.is_contiguous():
-        return cols
-    s0, s1, s2 = x.stride()
-    pitch = s1 if batch > 1 else (s0 if seq > 1 else cols)
-    if (cols > 1 and s2 != 1) or pitch < cols or (seq > 1 and batch > 1 and s0 != batch * s1):
-        raise ValueError(f"{name}: unsupported strides {tuple(x.stride())} for shape {tuple(shape)}")
-    return pitch
-
-
-def _state(h, name: str, batch: int, hidden: int, index: int) -> int:
-    """Address of a contiguous float32 tensor [batch, hidden]."""
-    if _lib.require_f32(h, name) != index or h.shape != (batch, hidden) or not h.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {(batch, hidden)} on cuda:{index}")
-    return h.data_ptr()
-
-
-def _lengths(lengths, batch: int, index: int):
-    """lengths, checked to be a contiguous int32 tensor [batch]."""
-    import torch
-    if lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.get_device() != index or \
-            not lengths.is_contiguous():
-        raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on cuda:{index}")
-    return lengths
-
-
-def _scan_args(gates, h0, lengths, candidate):
-    """(device index, seq, batch, hidden, gate pitch, h0, lengths, candidate), the last three as the C entry points take them."""
-    index = _lib.require_f32(gates, "gates")
-    if gates.dim() != 3 or gates.shape[2] % 2:
-        raise ValueError("gates must be [seq, batch, 2 * hidden]")
-    seq, batch, cols = gates.shape
-    hidden = cols // 2
-    if max(seq, batch, cols) > 0x7fffffff:
-        raise ValueError("gates: size > 2^31 - 1")
-    if candidate not in CANDIDATES:
-        raise ValueError(f"candidate must be one of {sorted(CANDIDATES)} (got {candidate!r})")
-    if lengths is not None:
-        lengths = _lengths(lengths, batch, index).data_ptr()
-    return (index, seq, batch, hidden, cols if gates.is_contiguous() else _step_rows(gates, "gates", gates.shape, index),
-            _state(h0, "h0", batch, hidden, index) if h0 is not None else None, lengths, CANDIDATES[candidate])
+def _candidate(name: str) -> int:
+    if name not in CANDIDATES:
+        raise ValueError(f"candidate must be one of {sorted(CANDIDATES)} (got {name!r})")
+    return CANDIDATES[name]
 
 
 def gated_scan(gates, h0=None, *, lengths=None, reverse: bool = False, candidate: str = "tanh", out=None, h_n=None,
@@ -279,19 +238,7 @@ def gated_scan(gates, h0=None, *, lengths=None, reverse: bool = False, candidate
     batch, hidden] may have a pitch; h_n [batch, hidden] may be h0 itself.
     Runs asynchronously on `stream` (default: torch's current stream).
     """
-    index, seq, batch, hidden, ld, h0p, lenp, cand = _scan_args(gates, h0, lengths, candidate)
-    if out is None:
-        out, ld_out = _lib.empty(gates, (seq, batch, hidden), stream), hidden
-    else:
-        ld_out = _step_rows(out, "out", (seq, batch, hidden), index)
-    if h_n is None:
-        h_n = _lib.empty(gates, (batch, hidden), stream)
-        h_np = h_n.data_ptr()
-    else:
-        h_np = _state(h_n, "h_n", batch, hidden, index)
-    _lib.call(index, stream, _lib.load().jst_scan_forward, gates.data_ptr(), ld, seq, batch, hidden, h0p, lenp, reverse,
-              cand, out.data_ptr(), ld_out, h_np)
-    return out, h_n
+    return _lib.calls().scan_forward(gates, h0, lengths, reverse, _candidate(candidate), out, h_n, stream)
 
 
 def gated_scan_backward(gates, out, dout, h0=None, *, dh_n=None, lengths=None, reverse: bool = False,
@@ -301,19 +248,7 @@ def gated_scan_backward(gates, out, dout, h0=None, *, dh_n=None, lengths=None, r
     dL/dh_n (either may be None: zero).  dgates is [seq, batch, 2 * hidden], 0
     behind a sequence's end; dh0 is None when h0 is.
     """
-    index, seq, batch, hidden, ld, h0p, lenp, cand = _scan_args(gates, h0, lengths, candidate)
-    ld_out = _step_rows(out, "out", (seq, batch, hidden), index)
-    ld_dout = _step_rows(dout, "dout", (seq, batch, hidden), index) if dout is not None else hidden
-    if dgates is None:
-        dgates, ld_dg = _lib.empty(gates, (seq, batch, 2 * hidden), stream), 2 * hidden
-    else:
-        ld_dg = _step_rows(dgates, "dgates", (seq, batch, 2 * hidden), index)
-    dh0 = _lib.empty(gates, (batch, hidden), stream) if h0 is not None else None
-    _lib.call(index, stream, _lib.load().jst_scan_backward, gates.data_ptr(), ld, seq, batch, hidden, h0p, lenp, reverse,
-              cand, out.data_ptr(), ld_out, dout.data_ptr() if dout is not None else None, ld_dout,
-              _state(dh_n, "dh_n", batch, hidden, index) if dh_n is not None else None, dgates.data_ptr(), ld_dg,
-              dh0.data_ptr() if dh0 is not None else None)
-    return dgates, dh0
+    return _lib.calls().scan_backward(gates, out, dout, h0, dh_n, lengths, reverse, _candidate(candidate), dgates, stream)
 
 
 class GatedRNN(_LayerDropout):
@@ -330,8 +265,7 @@ class GatedRNN(_LayerDropout):
                  batch_first: bool = False, candidate: str = "tanh", device="cuda", generator=None,
                  dropout: float = 0.0, seed: int = 0):
         import torch
-        if candidate not in CANDIDATES:
-            raise ValueError(f"candidate must be one of {sorted(CANDIDATES)} (got {candidate!r})")
+        _candidate(candidate)  # refuses other names
         self._init_dropout(dropout, seed)
         self.input_size, self.hidden_size, self.num_layers = input_size, hidden_size, num_layers
         self.bidirectional, self.batch_first, self.candidate = bidirectional, batch_first, candidate
@@ -387,7 +321,9 @@ class GatedRNN(_LayerDropout):
         x = x.contiguous()
         seq, batch, H, dirs = x.shape[0], x.shape[1], self.hidden_size, len(self._suffixes())
         if train and lengths is not None:  # rows behind a sequence meet dgates of 0 in the weights' gradient
-            behind = torch.arange(seq, device=x.device)[:, None] >= _lengths(lengths, batch, x.get_device())
+            if lengths.shape != (batch,) or lengths.device != x.device:
+                raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on {x.device}")
+            behind = torch.arange(seq, device=x.device)[:, None] >= lengths
             x = x.masked_fill(behind[..., None], 0.0)
         if h0 is not None and (tuple(h0.shape) != (self.num_layers * dirs, batch, H) or not h0.is_contiguous()):
             raise ValueError("h0 must be a contiguous [num_layers * num_directions, batch, hidden]")

@@ -136,21 +136,6 @@ def test_python_entry_points_refuse_host_tensors():
             call()
 
 
-def test_sizes_past_32_bits_are_refused(monkeypatch):
-    """The C entry points count rows in 32 bits: a larger tensor must not wrap to a smaller one."""
-    import torch
-
-    from jstorch_b200 import quant, rnn
-    monkeypatch.setattr(_lib, "require_f32", lambda x, name: 0)
-    monkeypatch.setattr(quant, "_require_i8", lambda x, name: 0)
-    rows = torch.zeros((2 ** 32 + 4, 0))
-    for call in (lambda: quant.quantize_rows(rows), lambda: quant.linear_i8(rows, rows[:3], rows[:3, 0:]),
-                 lambda: quant.gemm_i8(rows[:3], rows, rows, rows), lambda: rnn.gated_scan(rows[:, None]),
-                 lambda: rnn.gated_scan(rows[None])):
-        with pytest.raises(ValueError, match="size >"):
-            call()
-
-
 # ------------------------------------------------------------------ the oracle
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("tanh", [False, True])

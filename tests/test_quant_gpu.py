@@ -348,3 +348,16 @@ def test_refusals():
         quant.gemm_i8(q.to(torch.uint8), q, s, s)
     with pytest.raises(TypeError):
         quant.linear_i8(x.half(), q, s)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C entry points count rows in 32 bits: a larger tensor must not wrap to a smaller one."""
+    import torch
+    from jstorch_b200 import quant
+    rows = torch.zeros((2 ** 32 + 4, 0), device="cuda")
+    q = rows.to(torch.int8)
+    one = torch.ones(3, device="cuda")
+    for call in (lambda: quant.quantize_rows(rows), lambda: quant.linear_i8(rows, q[:3], one),
+                 lambda: quant.linear_i8(rows[:3], q, one), lambda: quant.gemm_i8(q[:3], q, one, one)):
+        with pytest.raises(ValueError, match="size >"):
+            call()

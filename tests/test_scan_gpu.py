@@ -266,3 +266,13 @@ def test_refusals():
                  lambda: rnn.gated_scan_backward(g, out, out, dgates=g)):
         with pytest.raises(JstError, match="overlap"):
             call()
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C entry points count rows in 32 bits: a larger tensor must not wrap to a smaller one."""
+    import torch
+    from jstorch_b200 import rnn
+    rows = torch.zeros((2 ** 32 + 4, 0), device="cuda")
+    for call in (lambda: rnn.gated_scan(rows[:, None]), lambda: rnn.gated_scan(rows[None])):
+        with pytest.raises(ValueError, match="size >"):
+            call()
