@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(1024)
 // SMs: each SM reads as much (1024 x 8192: 5.8 us, packed into full blocks 6.2;
 // 128 x 4096: 3.5 and 3.8).
 // Two rows a warp and four pieces of each in flight: 8192 x 8192 in 15.7 us
-// (4.1 TB/s; a row maximum of as many bytes takes 14.6), with one row 16.8 and
+// (4.3 TB/s; a row maximum of as many bytes takes 14.6), with one row 16.8 and
 // with four 23.7; quantising the token here adds nothing, a launch of its own 4.
 constexpr int kOneThreads = 256;
 constexpr int CH = 2;
