@@ -20,7 +20,8 @@
 //               a 32-entry table in shared memory), bias, ReLU, then a TMA
 //               store of the 32 x 32 block (16-byte aligned C), or row by row.
 //
-// gemm_i8_tokens_kernel: up to 64 tokens.  The roles are exchanged (C[s, r]):
+// gemm_i8_tokens_kernel: up to 64 tokens, or 64 at a time where tiles are few and
+// K is long.  The roles are exchanged (C[s, r]):
 // the 128-row side of the instruction holds channels, of which there are
 // plenty, and the other the tokens, padded to 16, 32 or 64 instead of 128.  The
 // call is a read of the weight, so it has to come from every SM: a cluster of
@@ -584,6 +585,7 @@ __global__ void __launch_bounds__(TOK_THREADS)
     const int kb0 = rank * p.kb_per_rank;
     const int num_kb = max(0, min((p.K + BK - 1) / BK - kb0, p.kb_per_rank));
     const int own = C::T >> p.cluster_log2, own0 = rank * own;  // the tokens whose sums meet in this CTA: a multiple of 4
+    const int m0 = blockIdx.y * C::T, tokens = p.tokens - m0;   // FP32: m0 is 0
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -606,7 +608,8 @@ __global__ void __launch_bounds__(TOK_THREADS)
     const uint32_t tmem_base = *tmem_slot;
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    if (!C::FP32 && threadIdx.x < own) token_scale[threadIdx.x] = own0 + threadIdx.x < p.tokens ? __ldg(p.token_scale + own0 + threadIdx.x) : 0.0f;
+    if (!C::FP32 && threadIdx.x < own) 
+        token_scale[threadIdx.x] = own0 + (int)threadIdx.x < tokens ? __ldg(p.token_scale + m0 + own0 + threadIdx.x) : 0.0f;
     if (cluster > 1) {  // nobody writes another's shared memory before that one runs
         ptx::cluster_arrive();
         ptx::cluster_wait();
@@ -620,7 +623,7 @@ __global__ void __launch_bounds__(TOK_THREADS)
                 uint8_t* st = smem + s * C::STAGE_BYTES;
                 ptx::mbar_arrive_expect_tx(&full_bar[s], C::STAGE_BYTES);
                 ptx::tma_load_3d(st, &tm_w, &full_bar[s], (kb0 + kb) * BK, n0, 0);
-                if (!C::FP32) ptx::tma_load_3d(st + C::R_BYTES, &tm_x, &full_bar[s], (kb0 + kb) * BK, 0, 0);
+                if (!C::FP32) ptx::tma_load_3d(st + C::R_BYTES, &tm_x, &full_bar[s], (kb0 + kb) * BK, m0, 0);
             }
         }
         __syncwarp();
@@ -656,7 +659,7 @@ __global__ void __launch_bounds__(TOK_THREADS)
             // this lane's channel: its partial sums of the tokens, four at a
             // time, to the CTA that owns those
 #pragma unroll 1
-            for (int c = 0; c < C::T && c < p.tokens; c += 16) {
+            for (int c = 0; c < C::T && c < tokens; c += 16) {
                 uint32_t r[16];
                 if (num_kb > 0) {
                     ptx::tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(q * 32) << 16) + c, r);
@@ -691,8 +694,8 @@ __global__ void __launch_bounds__(TOK_THREADS)
         const int row = (warp & 3) * 32 + lane, n = n0 + row;
         if (n < p.channels) {
             const float cs = __ldg(p.channel_scale + n), bias = p.bias ? __ldg(p.bias + n) : 0.0f;
-            float* out = p.C + (int64_t)own0 * p.ldc + n;
-            for (int i = 0; i < own && own0 + i < p.tokens; i += 4) {
+            float* out = p.C + (int64_t)(m0 + own0) * p.ldc + n;
+            for (int i = 0; i < own && own0 + i < tokens; i += 4) {
                 int4 sum = make_int4(0, 0, 0, 0);
                 for (int o = 0; o < cluster; ++o) {
                     const int4 v = *reinterpret_cast<const int4*>(exchange + (o * BM + row) * own + i);
@@ -701,7 +704,7 @@ __global__ void __launch_bounds__(TOK_THREADS)
                 const int v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (own0 + i + j < p.tokens)
+                    if (own0 + i + j < tokens)
                         out[(i + j) * p.ldc] = i8_finish(v[j], token_scale[i + j], cs, p.bias != nullptr, bias, p.relu);
             }
         }
@@ -830,9 +833,9 @@ static int launch_tokens(const CUtensorMap& w, const CUtensorMap& x, const TokPa
         }
     }
     const int cluster = 1 << p.cluster_log2;
-    const unsigned grid = (unsigned)((p.channels + BM - 1) / BM * cluster);
+    const dim3 grid((unsigned)((p.channels + BM - 1) / BM * cluster), (unsigned)((p.tokens + Cf::T - 1) / Cf::T));
     ProfScope prof(st, KID_GEMM_I8);
-    if (launch_dependent_cluster(gemm_i8_tokens_kernel<Cf>, dim3(grid), dim3(TOK_THREADS), cluster, Cf::SMEM_BYTES, st,
+    if (launch_dependent_cluster(gemm_i8_tokens_kernel<Cf>, grid, dim3(TOK_THREADS), cluster, Cf::SMEM_BYTES, st,
                                  w, x, p) != cudaSuccess)
         return set_status(JST_ERR_CUDA, "gemm_i8_tokens_kernel launch failed");
     return JST_OK;
@@ -841,6 +844,24 @@ static int launch_tokens(const CUtensorMap& w, const CUtensorMap& x, const TokPa
 // The pitch of a single row is never used, but a map wants a multiple of 16 bytes.
 static bool make_operand_map(CUtensorMap* m, const int8_t* x, int rows, int K, int64_t ld, int box_rows) {
     return make_map(m, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, rows, rows == 1 ? ((int64_t)K + 15) / 16 * 16 : ld, box_rows);
+}
+
+static int64_t tokens_tiles(const I8Args& a, int T) { return (int64_t)((a.N + BM - 1) / BM) * ((a.M + T - 1) / T); }
+
+// CTAs that share a tile of T tokens: as many as the SMs take (two CTAs of up to
+// 32 tokens fit one), with a k-slab and four tokens at least each (16 tokens,
+// 4096 x 4096: 15.6 us alone, 10.4 with two, 7.9 with four; 16, 2048 x 512:
+// 5.3, 4.8, 4.2; 64, 8192 x 8192: 34.1, 21.6, and 28.4 with four, which no
+// longer run at the same time).  A cluster keeps to one GPC, so the last SMs of
+// each stay empty: of clusters of 4, 33 run at once and 34 do not (64, 4224 x 4096
+// 11.1 us, 4352 x 4096 18.7, with two 14.1), of 8, 15 and not 16 (1920 x 4096 9.1,
+// 2048 x 4096 15.6, with four 9.6).
+static int tokens_cluster_log2(const I8Args& a, int T) {
+    const int64_t tiles = tokens_tiles(a, T);
+    const int slabs = (a.K + BK - 1) / BK, room = sm_count() * (T <= 32 ? 2 : 1), percent[] = {100, 88, 80};
+    int lg = 0;
+    while (lg < 3 && (8 << lg) <= T && (tiles << (lg + 1)) <= room * percent[lg] / 100 && (2 << lg) <= slabs) ++lg;
+    return lg;
 }
 
 // x: the tokens in fp32 (gemm_i8_tc_takes_fp32), or null.
@@ -856,14 +877,7 @@ static int run_tokens(const I8Args& a, const float* x, int64_t ldx, cudaStream_t
     p.channel_scale = a.b_scale; p.token_scale = a.a_scale;
     p.bias = a.bias; p.relu = a.relu;
     p.err = device_error_word();
-    // CTAs that share a tile: as many as the SMs take (two CTAs of up to 32
-    // tokens fit one), with a k-slab and four tokens at least each (16 tokens,
-    // 4096 x 4096: 15.6 us alone, 10.4 with two, 7.9 with four; 16, 2048 x 512:
-    // 5.3, 4.8, 4.2; 64, 8192 x 8192: 34.1, 21.6, and 28.4 with four, which no
-    // longer run at the same time)
-    const int tiles = (a.N + BM - 1) / BM, slabs = (a.K + BK - 1) / BK, room = sm_count() * (T <= 32 ? 2 : 1);
-    int lg = 0;
-    while (lg < 3 && (8 << lg) <= T && (tiles << (lg + 1)) <= room && (2 << lg) <= slabs) ++lg;
+    const int lg = tokens_cluster_log2(a, T), slabs = (a.K + BK - 1) / BK;
     p.cluster_log2 = lg;
     p.kb_per_rank = (slabs + (1 << lg) - 1) >> lg;
     p.x = x;
@@ -895,6 +909,13 @@ static int run_aligned(const I8Args& a, cudaStream_t s) {
             bn = k.cols;
         }
     }
+    // Few tiles and a long K: the kernel of few tokens, 64 at a time, whose clusters
+    // share K, at 350 ns a k-slab and an exchange that shrinks with a CTA's part of
+    // the tile (us: 200 x 300 x 8192 takes 10.0, in tiles 22.1, 200 x 1024 x 4096 10.2 and
+    // 13.0; 1000 x 1024 x 8192 would take 29.0, in tiles 22.9).
+    const int lg = tokens_cluster_log2(a, 64), slabs = (a.K + BK - 1) / BK;
+    const int exchange_ns[] = {7650, 6350, 5950, 4450};
+    if (lg > 0 && exchange_ns[lg] + (int64_t)((slabs + (1 << lg) - 1) >> lg) * 350 < best) return run_tokens(a, nullptr, 0, s);
     const bool pair = bn == 256;
     Params p{};
     p.R = a.M; p.S = a.N; p.K = a.K;

@@ -45,7 +45,7 @@ def _aligned(x):
 
 
 SIZES = [(1, 1, 1), (1, 7, 3), (1, 128, 64), (1, 1000, 4096), (1, 20, 1024), (1, 21, 1025), (1, 40, 8192), (1, 33, 8195),
-         (1, 50, 20001), (1, 1024, 8208), (1, 1301, 20000), (2, 1, 5), (6, 3000, 700), (16, 5, 640), (40, 130, 2050), (64, 1500, 129), (65, 300, 40), (2, 33, 100), (3, 64, 16), (4, 129, 515), (5, 256, 512),
+         (1, 50, 20001), (1, 1024, 8208), (65, 1, 8191), (130, 257, 8000), (999, 65, 7000), (200, 2048, 4096), (1, 1301, 20000), (2, 1, 5), (6, 3000, 700), (16, 5, 640), (40, 130, 2050), (64, 1500, 129), (65, 300, 40), (2, 33, 100), (3, 64, 16), (4, 129, 515), (5, 256, 512),
          (7, 31, 77), (8, 512, 1024), (9, 100, 260), (15, 65, 48), (16, 130, 1000), (17, 64, 128), (31, 200, 96),
          (33, 257, 129), (64, 64, 64), (100, 300, 1031), (127, 128, 127), (128, 256, 128), (129, 257, 144),
          (200, 513, 2000), (256, 1024, 784), (300, 70, 6000), (513, 129, 17), (1000, 5, 300)]
