@@ -940,7 +940,7 @@ static int run_aligned(const I8Args& a, cudaStream_t s) {
 }  // namespace i8
 
 // Up to 16 tokens of so few values that one launch beats two: such calls wait
-// for the host, which spends 5.1 us on this one and 7.8 on a quantisation, its
+// for the host, which spends 4.4 us on this one and 7.5 on a quantisation, its
 // workspace and the product (5 x 2048 x 512; on the device alone 6.7 and 5.6,
 // and 16 x 1024 x 1024, 10.6 and 6.3).  The weight needs no copy.
 bool gemm_i8_tc_takes_fp32(const I8Args& a) {
