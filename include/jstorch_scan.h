@@ -20,6 +20,8 @@ enum { JST_SCAN_TANH = 0, JST_SCAN_IDENTITY = 1 };
 /*
  * For every sequence b and unit j, over the steps of the sequence in order:
  *   z = sigmoid(a)    n = tanh(c) or c    h_t = z * h_{t-1} + (1 - z) * n
+ * z and 1 - z are 0 where they are below 2^-126 (a beyond 87.3 either way): such a
+ * gate keeps nothing of the state, whatever its size, or takes nothing of n.
  *   gates    row (t, b) at gates + (t * batch + b) * ld_gates: a in columns
  *            [0, hidden), c in [hidden, 2 * hidden); ld_gates >= 2 * hidden
  *            (every pitch is below 2^24)

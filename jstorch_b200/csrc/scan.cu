@@ -109,13 +109,13 @@ __device__ __forceinline__ F<V> operator-(const F<V>& a) {  // folds into the op
     return r;
 }
 
-// exp(-x) as 2^(-x log2 e), |x| <= 127: the rounding error of that product (and
-// of log2 e) is found by a fused multiply-add and put back to first order, so
-// what is left is the 2^-22 of the power and a rounding.  Results below 2^-126
-// flush to 0.
-template <int V>
+// exp(-TIMES x) as 2^(-x TIMES log2 e), TIMES 1 or 2 and |TIMES x| <= 127: the rounding
+// error of that product (and of log2 e) is found by a fused multiply-add and put back
+// to first order, so what is left is the 2^-22 of the power and a rounding.  Results
+// below 2^-126 flush to 0.
+template <int TIMES, int V>
 __device__ __forceinline__ F<V> exp_minus(const F<V>& x) {
-    const float log2e = 1.44269502162933349609375f, log2e_rest = 1.92596299112661746887e-8f;
+    const float log2e = TIMES * 1.44269502162933349609375f, log2e_rest = TIMES * 1.92596299112661746887e-8f;
     const F<V> t = x * all<V>(-log2e);
     F<V> r = fma(x, all<V>(-log2e), -t);
     r = fma(x, all<V>(-log2e_rest), r) * all<V>(0.693147180559945309f);
@@ -145,17 +145,20 @@ __device__ __forceinline__ float at_most(float x, float hi) {
 
 // z = 1 / (1 + e) and 1 - z = e z with e = exp(-a): neither loses digits where
 // it is small.  The reciprocal takes one Newton step: its ulp leans to one side,
-// and a state that is remembered for a thousand steps would add it up.  a is kept within [-87, 127], where e is a number and z is
-// positive: below, z is held at 2^-126 (1.65e-38), which a state's share of
-// the next one cannot show beside anything but 0.
+// and a state that is remembered for a thousand steps would add it up.  A gate
+// whose z or 1 - z is no normal number (below 2^-126: |a| > 87.33) is closed or open
+// altogether, and a closed one keeps nothing of a state of any size: a is clamped
+// where 1 + e is above 2^126, whose reciprocal flushes to 0.  The residual q, at most 2^-22
+// elsewhere, is 1 then, and rounded to an integer it is the 1 - z that e z lacks.
 template <int V>
 __device__ __forceinline__ void gate(const F<V>& a, F<V>& z, F<V>& rest) {
+    constexpr float shift = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
     F<V> x;
 #pragma unroll
-    for (int i = 0; i < V; ++i) x.v[i] = at_most(at_least(a.v[i], -87.0f), 127.0f);
-    const F<V> e = exp_minus(x), d = e + all<V>(1.0f), r = reciprocal(d);
-    z = fma(r, fma(-d, r, all<V>(1.0f)), r);
-    rest = e * z;
+    for (int i = 0; i < V; ++i) x.v[i] = at_most(at_least(a.v[i], -88.0f), 127.0f);
+    const F<V> e = exp_minus<1>(x), d = e + all<V>(1.0f), r = reciprocal(d), q = fma(-d, r, all<V>(1.0f));
+    z = fma(r, q, r);
+    rest = fma(e, z, (q + all<V>(shift)) + all<V>(-shift));
 }
 
 // tanh(c) = (1 - t) / (1 + t) of |c| with t = exp(-2 |c|), and below 0.6, where
@@ -169,7 +172,7 @@ __device__ __forceinline__ F<V> candidate(const F<V>& c) {
         F<V> x;
 #pragma unroll
         for (int i = 0; i < V; ++i) x.v[i] = at_most(fabsf(c.v[i]), 60.0f);
-        const F<V> t = exp_minus(x + x);
+        const F<V> t = exp_minus<2>(x);
         const F<V> far = (all<V>(1.0f) + -t) * reciprocal(t + all<V>(1.0f));
         const F<V> q = c * c;
         F<V> p = fma(q, all<V>(-0.005895157810300589f), all<V>(0.020795971155166626f));
@@ -185,9 +188,8 @@ __device__ __forceinline__ F<V> candidate(const F<V>& c) {
 }
 
 // A product of z in (0, 1) underflows to 0 after some hundred steps, and 0 times
-// an infinite state would be NaN where step by step it stays infinite: as no z
-// is 0, products are kept at 2^-149 at least (2^-149 of the state, far below a
-// rounding of what is added to it).
+// an infinite state would be NaN where step by step it stays infinite: unless a z
+// is 0, products are kept at 2^-149 at least, which is a rounding of theirs.
 constexpr float kTiny = 1.40129846432481707e-45f;
 
 template <int V>
@@ -355,7 +357,12 @@ struct Steps {
             A = A * z[i];
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) A.v[v] = fmaxf(A.v[v], kTiny);
+        for (int v = 0; v < V; ++v) {
+            float least = kTiny;  // 0 where a z is
+#pragma unroll
+            for (int i = 0; i < K; ++i) least = fminf(least, z[i].v[v]);
+            A.v[v] = fmaxf(A.v[v], least);
+        }
     }
     template <bool ALL>
     __device__ __forceinline__ F<V> finish_part(F<V> e, int seq, const Channels<BWD, V>& w, int64_t s0) const {
@@ -518,9 +525,10 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
                 for (int q = 1; q < S; ++q) {
                     const Pair<V> f = warps[parity][q][lane];
                     run.B = fma(f.A, run.B, f.B);
-                    run.A = f.A * run.A;
+                    const F<V> A = f.A * run.A;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) run.A.v[v] = fmaxf(run.A.v[v], kTiny);
+                    for (int v = 0; v < V; ++v)  // 0 where a factor is
+                        run.A.v[v] = fmaxf(A.v[v], fminf(fminf(f.A.v[v], run.A.v[v]), kTiny));
                 }
                 // A block is two rounds ahead of another's reads of these places
                 // only after that other has sent the round between: it has read them.
@@ -597,7 +605,8 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 //     over warps 5.7 / 8.8; 16 x 64 x 1024: 6.2 / 8.0, split 6.1 / 10.1;
 //     128 x 256 x 1024: 71 / 136, split 84 / 150).
 //   * Many tiles of a short axis: small blocks, of which many fit an SM
-//     (64 x 64 x 1024: 12.5 / 19.2; in blocks of 8 warps x 8 steps 15.1 / 24.8).
+//     (64 x 64 x 1024: 12.3 / 18.5, 33 x 70 x 1024: 11.3 / 14.4 in blocks of 2 warps x 8
+//     steps; 4 x 4: 13.7 / 18.9, 12.7 / 16.4; 8 x 8: 15.1 / 24.8 for the first).
 //   * Otherwise 64 steps a block and round, 8 a lane (2048 x 16 x 1024 forward
 //     79, with 4 steps a lane 100; backward 4 warps x 8 steps 138, 8 x 8 146,
 //     4 x 4 200), and where the tiles leave SMs empty, clusters that share a
@@ -622,7 +631,7 @@ int run_scan(const ScanArgs& p, cudaStream_t s) {
         scan_serial_kernel<BWD, TANH, V, 4><<<(unsigned)grid, kSerialThreads, 0, s>>>(p);
         return JST_OK;
     }
-    if (p.seq <= 64 && tiles >= 4 * sms) return launch_tiled<BWD, TANH, V, 4, 4, BWD ? 5 : 7>(p, 1, s);
+    if (p.seq <= 64 && tiles >= 4 * sms) return launch_tiled<BWD, TANH, V, 2, 8, BWD ? 4 : 8>(p, 1, s);
     const bool uneven = p.lengths && p.seq > 1024;
     if (BWD && V == 2 && tiles >= sms && !uneven) return launch_tiled<BWD, TANH, V, 4, 8, 1>(p, 1, s);
     constexpr int blocks_per_sm = BWD && V == 2 ? 1 : 2;

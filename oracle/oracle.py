@@ -455,21 +455,24 @@ def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, 
 
     The bounds carry first-order rounding errors through the recurrence, u =
     2^-24.  One exponential e of -a (a power of two to 2^-22 = 4u, and 2
-    roundings) gives z = 1 / (1 + e) (its sum 1u, the reciprocal 1 ulp = 2u, and
-    e / (1 + e) = 1 - z of e's error) and 1 - z as e z (z of e's error remains,
-    z's roundings, 1u), so the larger of z and 1 - z is off by 5u + 6u of the
-    smaller, and the smaller by 14u, relative.  tanh as (1 - t) / (1 + t) from t = exp(-2 |c|)
+    roundings: 6u) gives z = 1 / (1 + e) (the sum 1u, the reciprocal after a Newton step
+    1u) and 1 - z as e z (1u), so the larger of z and 1 - z is off by 3u + 6u of
+    the smaller, and the smaller by 9u, relative.  tanh as (1 - t) / (1 + t) from t = exp(-2 |c|)
     <= 0.3 (|c| >= 0.6) has 6u t / (1 - t) and 6u t / (1 + t) of t's error, two
     sums, a reciprocal and a product: 9u; nearer to 0 it is a polynomial's 3u.
+    Where |a| > 87.3 the smaller of z and 1 - z is below 2^-126 and may be 0: its size
+    times what it would have met.
     Each step then rounds a product and a sum, and a scan that composes steps
     (products of z) rounds once more a step: 3u.  The few compositions of a
-    scan's tree add 16u once.  An exponential below 2^-126 may flush to 0, z may
-    be held at 1.5 2^-126 and products round to a grid of 2^-149, whatever their
-    size, which the factors that they meet carry on: 2^-125 a step times those.
+    scan's tree add 16u once.  Below 2^-126 numbers round to a grid of 2^-149,
+    whatever their size: a gate by 1 of its steps, its complement by 1, products of gates
+    and what they meet by half of one each, which the factors carry on: 2^-146 a
+    step times the largest state so far (a product of gates may span all steps
+    before), candidate or gradient.
     m and g are the magnitudes (the same sums of
     absolute values) that these relative errors apply to.
     """
-    u, tiny = 2.0 ** -24, 2.0 ** -125
+    u, tiny = 2.0 ** -24, 2.0 ** -146
     gates = np.asarray(gates, dtype=np.float64)
     seq, batch, hidden = gates.shape[0], gates.shape[1], gates.shape[2] // 2
     length = np.full(batch, seq) if lengths is None else np.clip(np.asarray(lengths), 0, seq)
@@ -480,21 +483,24 @@ def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, 
     big, small = 1 / (1 + e), e / (1 + e)
     z, rest = np.where(a >= 0, big, small), np.where(a >= 0, small, big)
     n = np.tanh(c) if tanh else c
-    of_big = 5 + 6 * small
-    cz, cr = np.where(a >= 0, of_big, 14.0), np.where(a >= 0, 14.0, of_big)
+    lost = np.where(np.abs(a) > 87.3, small, 0.0)
+    of_big = 3.01 + 6 * small
+    cz, cr = np.where(a >= 0, of_big, 9.01), np.where(a >= 0, 9.01, of_big)
     cn = 9.0 if tanh else 0.0
     times = range(seq - 1, -1, -1) if reverse else range(seq)
     h = np.zeros((batch, hidden)) if h0 is None else np.asarray(h0, dtype=np.float64)
     m, err = np.abs(h), np.zeros((batch, hidden))
+    most = m
     before, before_m, before_e = np.empty_like(z), np.empty_like(z), np.empty_like(z)
     out, out_e = np.zeros_like(z), np.zeros_like(z)
     for t in times:
         k = inside[t][:, None]
         before[t], before_m[t], before_e[t] = h, m, err
         err = np.where(k, z[t] * err + u * ((cz[t] + 3) * z[t] * m + (cr[t] + cn + 3) * rest[t] * np.abs(n[t]))
-                       + tiny * (m + np.abs(n[t]) + 1), err)
+                       + tiny * (most + np.abs(n[t]) + 1) + lost[t] * (m + np.abs(n[t])), err)
         h = np.where(k, z[t] * h + rest[t] * n[t], h)
         m = np.where(k, z[t] * m + rest[t] * np.abs(n[t]), m)
+        most = np.maximum(most, m)
         out[t], out_e[t] = np.where(k, h, 0.0), np.where(k, err + 16 * u * m, 0.0)
     r = {"out": (out, out_e), "h_n": (h, err + 16 * u * m)}
     if not with_grads:
@@ -502,21 +508,23 @@ def scan_f64(gates, h0=None, lengths=None, reverse=False, tanh=True, dout=None, 
     dout = np.zeros_like(z) if dout is None else np.asarray(dout, dtype=np.float64)
     g = np.zeros((batch, hidden)) if dh_n is None else np.asarray(dh_n, dtype=np.float64)
     gm, ge = np.abs(g), np.zeros((batch, hidden))
+    most = gm
     dgates, dgates_e = np.zeros_like(gates), np.zeros_like(gates)
     for t in reversed(times):
         k = inside[t][:, None]
         d = np.where(k, dout[t], 0.0)
         G, Gm = g + d, gm + np.abs(d)
         Ge = ge + 17 * u * Gm
+        most = np.maximum(most, Gm)
         diff = before[t] - n[t]
         diff_e = before_e[t] + 16 * u * before_m[t] + cn * u * np.abs(n[t]) + u * np.abs(diff)
         slope = z[t] * rest[t]
         dn = rest[t] * ((1 - n[t] ** 2) if tanh else 1.0)
         dgates[t] = np.where(k, np.concatenate([G * diff * slope, G * dn], axis=1), 0.0)
         dgates_e[t] = np.where(k, np.concatenate([
-            tiny * (Gm + 1) * (np.abs(diff) + 1) + Ge * np.abs(diff) * slope + Gm * slope * (diff_e + np.abs(diff) * (cz[t] + cr[t] + 3) * u),
-            tiny * (Gm + 1) + Ge * dn + Gm * (dn * (cr[t] + 3) * u + (rest[t] * 20 * u if tanh else 0.0))], axis=1), 0.0)
-        ge = np.where(k, z[t] * ge + u * (cz[t] + 4) * z[t] * Gm + tiny * (Gm + 1), ge)
+            (tiny * (Gm + 1) + lost[t] * Gm) * (np.abs(diff) + 1) + Ge * np.abs(diff) * slope + Gm * slope * (diff_e + np.abs(diff) * (cz[t] + cr[t] + 3) * u),
+            tiny * (Gm + 1) + lost[t] * Gm + Ge * dn + Gm * (dn * (cr[t] + 3) * u + (rest[t] * 20 * u if tanh else 0.0))], axis=1), 0.0)
+        ge = np.where(k, z[t] * ge + u * (cz[t] + 4) * z[t] * Gm + tiny * (most + 1) + lost[t] * Gm, ge)
         g, gm = np.where(k, z[t] * G, g), np.where(k, z[t] * Gm, gm)
     r["dgates"] = (dgates, dgates_e)
     r["dh0"] = (g, ge + 16 * u * gm)
