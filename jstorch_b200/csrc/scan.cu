@@ -4,7 +4,7 @@
 // and its gradients
 //   G_t = dout_t + z_{t+1} G_{t+1}      (last step: dout_t + dh_n)
 //   da_t = G_t (h_{t-1} - n_t) z_t (1 - z_t)
-//   dc_t = G_t (1 - z_t) (1 - n_t^2 or 1)      dh0 = z_0 G_0
+//   dc_t = G_t (1 - z_t) (dn/dc: 1 - n_t^2 or 1)      dh0 = z_0 G_0
 // Both are first-order recurrences  e' = A e + B  along one channel:
 //   forward  e = h,                A = z,  B = (1 - z) n
 //   backward e_t = z_{t+1} G_{t+1} (what the later steps hand back; dh_n at
@@ -161,19 +161,20 @@ __device__ __forceinline__ void gate(const F<V>& a, F<V>& z, F<V>& rest) {
     rest = fma(e, z, (q + all<V>(shift)) + all<V>(-shift));
 }
 
-// tanh(c) = (1 - t) / (1 + t) of |c| with t = exp(-2 |c|), and below 0.6, where
+// n = tanh(c) = (1 - t) / (1 + t) of |c| with t = exp(-2 |c|), and below 0.6, where
 // 1 - t would lose digits, c + c^3 P(c^2) with P of degree 4 fitted to the
-// relative error (0.05 of 2^-24).
-template <bool TANH, int V>
-__device__ __forceinline__ F<V> candidate(const F<V>& c) {
+// relative error (0.05 of 2^-24).  slope: dn/dc, which is 4 t / (1 + t)^2 (where n
+// rounds to 1 that keeps its digits, and 1 - n^2 has none) and below 0.6 1 - n^2.
+template <bool TANH, bool SLOPE, int V>
+__device__ __forceinline__ F<V> candidate(const F<V>& c, F<V>& slope) {
     if constexpr (!TANH) {
         return c;
     } else {
         F<V> x;
 #pragma unroll
         for (int i = 0; i < V; ++i) x.v[i] = at_most(fabsf(c.v[i]), 60.0f);
-        const F<V> t = exp_minus<2>(x);
-        const F<V> far = (all<V>(1.0f) + -t) * reciprocal(t + all<V>(1.0f));
+        const F<V> t = exp_minus<2>(x), w = reciprocal(t + all<V>(1.0f));
+        const F<V> far = (all<V>(1.0f) + -t) * w;
         const F<V> q = c * c;
         F<V> p = fma(q, all<V>(-0.005895157810300589f), all<V>(0.020795971155166626f));
         p = fma(p, q, all<V>(-0.053783830255270004f));
@@ -183,6 +184,11 @@ __device__ __forceinline__ F<V> candidate(const F<V>& c) {
         F<V> n;
 #pragma unroll
         for (int i = 0; i < V; ++i) n.v[i] = fabsf(c.v[i]) < 0.6f ? near.v[i] : copysignf(far.v[i], c.v[i]);
+        if (SLOPE) {
+            const F<V> near_slope = fma(-near, near, all<V>(1.0f)), far_slope = t * all<V>(4.0f) * w * w;
+#pragma unroll
+            for (int i = 0; i < V; ++i) slope.v[i] = fabsf(c.v[i]) < 0.6f ? near_slope.v[i] : far_slope.v[i];
+        }
         return n;
     }
 }
@@ -330,10 +336,11 @@ struct Steps {
         for (int i = 0; i < K; ++i) {
             F<V> rest;
             gate(r.a[i], z[i], rest);
-            const F<V> n = candidate<TANH>(r.c[i]);
+            F<V> slope;
+            const F<V> n = candidate<TANH, BWD>(r.c[i], slope);
             if (BWD) {
                 fa[i] = (r.h[i] + -n) * (z[i] * rest);
-                fc[i] = TANH ? rest * fma(-n, n, all<V>(1.0f)) : rest;
+                fc[i] = TANH ? rest * slope : rest;
                 add[i] = r.d[i];
             } else {
                 add[i] = rest * n;
