@@ -13,10 +13,9 @@ extern "C" {
 #endif
 
 /*
- * Quantise rows: scale[r] = max_k |x[r, k]| * (1 / 127), the reciprocal and the
- * product rounded to fp32, and q[r, k] = x[r, k] / scale[r] rounded to the
- * nearest integer (ties to even), within [-127, 127].  A row of zeros has scale
- * 0 and q = 0; a row that holds an infinity or a NaN has scale NaN and q = 0, so
+ * Quantise rows: scale[r] = max_k |x[r, k]| / 127 rounded to fp32, and q[r, k] =
+ * x[r, k] / scale[r] rounded to the nearest integer (ties to even), within
+ * [-127, 127].  A row of zeros has scale 0 and q = 0; a row that holds an infinity or a NaN has scale NaN and q = 0, so
  * every product of it is NaN (0 behind a ReLU, as in jst_gemm_ex).
  *   x  row r at x + r * ldx, ldx >= cols;   q  row r at q + r * ldq, ldq >= cols
  * rows and cols are at most 0x7fff0000; the arrays do not overlap.  The bytes of

@@ -31,13 +31,13 @@ __device__ __forceinline__ float i8_finish(int acc, float sa, float sb, bool has
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 __device__ __forceinline__ float row_scale(uint32_t peak) {
-    return peak < 0x7f800000u ? __fmul_rn(__uint_as_float(peak), 1.0f / 127.0f) : __uint_as_float(0x7fffffffu);
+    return peak < 0x7f800000u ? __fdiv_rn(__uint_as_float(peak), 127.0f) : __uint_as_float(0x7fffffffu);
 }
 // 1 / s, or 0 where the row quantises to zeros (s is 0 or NaN).
 __device__ __forceinline__ float row_inverse(float s) { return s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f; }
 
 // q = x / s to the nearest integer, ties to even, within [-127, 127], where s =
-// max|x| * (1 / 127) > 0, by a division in 64 bits.  (A call: it is rare.)
+// max|x| / 127 > 0, by a division in 64 bits.  (A call: it is rare.)
 static __device__ __noinline__ uint32_t quantize_exactly(float x, float s) {
     return (uint32_t)(uint8_t)(int8_t)fmin(fmax(rint((double)x / (double)s), -127.0), 127.0);
 }

@@ -11,8 +11,8 @@ from . import _lib
 
 
 def quantize_rows(x, *, stream=None):
-    """(q, scale) of a 2-D float32 CUDA tensor: scale[r] = max|x[r]| * (1 / 127)
-    in fp32, q[r] = x[r] / scale[r] to the nearest integer (ties to even) in int8.
+    """(q, scale) of a 2-D float32 CUDA tensor: scale[r] = max|x[r]| / 127
+    rounded to fp32, q[r] = x[r] / scale[r] to the nearest integer (ties to even) in int8.
     A row that holds an infinity or a NaN gets scale NaN.  The rows of q start
     at multiples of 16 bytes (q is a view when x has other widths), as
     gemm_i8 reads them in place.

@@ -571,13 +571,13 @@ def dropout_f32(x, p: float, seed: int, offset: int = 0) -> np.ndarray:
 
 # ------------------------------------------------------------ 8-bit product
 def quantize_rows(x):
-    """(q, scale) of fp32 rows: scale = max|x| * (1 / 127) in fp32, q = x / scale in
+    """(q, scale) of fp32 rows: scale = max|x| / 127 rounded to fp32, q = x / scale in
     fp64, to the nearest integer, ties to even; a row that is not finite has
     scale NaN and q = 0."""
     x = np.asarray(x, dtype=np.float32)
     peak = np.abs(x).max(axis=1, initial=np.float32(0.0))
     with np.errstate(invalid="ignore"):
-        scale = np.where(np.isfinite(peak), peak * (np.float32(1.0) / np.float32(127.0)), np.float32(np.nan)).astype(np.float32)
+        scale = np.where(np.isfinite(peak), peak / np.float32(127.0), np.float32(np.nan)).astype(np.float32)
     usable = np.isfinite(scale) & (scale > 0)
     s = np.where(usable, scale, np.float32(1.0)).astype(np.float64)
     v = np.where(usable[:, None], x, np.float32(0.0)).astype(np.float64) / s[:, None]
