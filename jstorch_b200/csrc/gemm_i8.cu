@@ -533,13 +533,21 @@ __device__ __forceinline__ void quantize_tokens(const TokParams& p, uint8_t* sme
         for (int i = 0; i < ROWS; ++i)
             peak[i] = max(max(max(peak[i], abs_bits(v[i].x)), max(abs_bits(v[i].y), abs_bits(v[i].z))), abs_bits(v[i].w));
     }
+    // A lane a row: the divisions of all rows at once (5 x 2048 x 512: one row after the other, 0.4 us more).
+    uint32_t of_mine = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const uint32_t of_row = __reduce_max_sync(0xffffffffu, peak[i]);
+        if (lane == i) of_mine = of_row;
+    }
+    const float my_scale = row_scale(of_mine), my_inverse = row_inverse(my_scale);
+    const int my_row = w + 4 * lane - own0;
+    if (lane < ROWS && my_row >= 0 && my_row < own) token_scale[my_row] = my_scale;
     float s[ROWS], inv[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int m = w + 4 * i;
-        s[i] = row_scale(__reduce_max_sync(0xffffffffu, peak[i]));
-        inv[i] = row_inverse(s[i]);
-        if (lane == 0 && m >= own0 && m < own0 + own) token_scale[m - own0] = s[i];
+        s[i] = __shfl_sync(0xffffffffu, my_scale, i);
+        inv[i] = __shfl_sync(0xffffffffu, my_inverse, i);
     }
 #pragma unroll 2
     for (int kb = 0; kb < num_kb; ++kb) {
