@@ -30,8 +30,8 @@ int jst_quantize_rows_i8(const float* x, int64_t ldx, int rows, int cols, int8_t
  *   A [M][K] int8 (tokens), row pitch lda >= K;  B [N][K] int8 (channels: an
  *   nn.Linear weight), row pitch ldb >= K;  C [M][N] fp32, row pitch ldc >= N.
  *   All int8 values are legal (-128 too).  The sum is exact (32-bit integers;
- *   K <= 131071); it is rounded to fp32 once and multiplied by the rounded
- *   product of the scales.
+ *   K <= 131071); it is rounded to fp32 once and multiplied by one scale after the
+ *   other, in an order that overflows or underflows only where the result does.
  *   a_scale [M], b_scale [N]; bias [N], required by the bias epilogues.
  *   epilogue: JST_EPI_NONE, JST_EPI_BIAS, JST_EPI_RELU or JST_EPI_BIAS_RELU.
  *   An operand whose address or pitch is not a multiple of 16 bytes is first

@@ -18,9 +18,15 @@ struct I8Args {
 };
 
 // The epilogue that every kernel of the product shares, so that they agree in
-// every bit: the sum rounded to fp32, the rounded product of the two scales.
+// every bit: the sum rounded to fp32, times the token's scale, times the
+// channel's; or times the channel's first where |acc sa|, |acc| <= 2^31, could
+// overflow.  (A whole number times a scale loses nothing to underflow, where the
+// product of two scales may: what meets the type's range is the result alone.)
+// One of the three factors is 1.
 __device__ __forceinline__ float i8_finish(int acc, float sa, float sb, bool has_bias, float bias, int relu) {
-    float v = __fmul_rn(__int2float_rn(acc), __fmul_rn(sa, sb));
+    const bool late = fabsf(sa) > 7.9228162514264338e28f;  // 2^96
+    float v = __fmul_rn(__int2float_rn(acc), late ? 1.0f : sa);
+    v = __fmul_rn(__fmul_rn(v, sb), late ? sa : 1.0f);
     if (has_bias) v = __fadd_rn(v, bias);
     return relu ? fmaxf(v, 0.0f) : v;
 }

@@ -586,13 +586,13 @@ def quantize_rows(x):
 
 def gemm_i8_f64(a, w, a_scale, w_scale, bias=None, relu=False):
     """(value, bound) of a_scale w_scale (a . w^T) + bias.  The integer sum is
-    exact; fp32 rounds it, the product of the scales and their product (3 half
-    steps) and the sum with the bias (1): 3u |product| + u |value|, and a scale
-    that underflows rounds by an absolute 2^-150."""
+    exact; fp32 rounds it and its products with the two scales (3 half
+    steps) and the sum with the bias (1): 3u |product| + u |value|, and a result
+    below the normal numbers rounds by an absolute 2^-150."""
     acc = np.asarray(a, dtype=np.float64) @ np.asarray(w, dtype=np.float64).T
     scale = np.asarray(a_scale, dtype=np.float64)[:, None] * np.asarray(w_scale, dtype=np.float64)[None, :]
     product = acc * scale
     value = product if bias is None else product + np.asarray(bias, dtype=np.float64)[None, :]
     u = 2.0 ** -24
-    bound = (3.001 * u * np.abs(product) + u * np.abs(value) + (np.abs(acc) + 1) * 2.0 ** -150) * 1.001
+    bound = (3.001 * u * np.abs(product) + u * np.abs(value) + 2.0 ** -149) * 1.001
     return (np.maximum(value, 0.0) if relu else value), bound

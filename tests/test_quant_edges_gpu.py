@@ -31,3 +31,22 @@ def test_scale_is_the_rounded_quotient():
     for rows in (1, 8, 70):
         y = quant.linear_i8(_dev(x[:rows]), _dev(np.eye(40, dtype=np.int8)), _dev(one)).cpu().numpy()
         np.testing.assert_array_equal(y, want[:rows].astype(np.float32) * scale[:rows, None])
+
+
+@pytest.mark.parametrize("M", [1, 5, 40, 100, 700])
+def test_scales_whose_product_leaves_the_type(M):
+    """A product of scales below 2^-126 or above 2^128 costs no digits, and no zero, of a result within the type."""
+    from jstorch_b200 import quant
+    rng = np.random.default_rng(M)
+    N, K = 300, 512
+    a, w = (rng.integers(-128, 128, (n, K), dtype=np.int8) for n in (M, N))
+    a[::3] = 0  # sums of 0
+    w[::5, 1:] = 0  # small sums
+    for sa, sw in ((1e-30, 1e-9), (1e-9, 1e-30), (1e-42, 1e30), (1e30, 1e-42), (3e38, 1e-9), (1e-9, 3e38), (1e20, 1e20), (1e38, 1e38)):
+        a_scale, w_scale = (np.full(n, s, np.float32) * rng.uniform(0.5, 1, n).astype(np.float32) for n, s in ((M, sa), (N, sw)))
+        value, bound = oracle.gemm_i8_f64(a, w, a_scale, w_scale)
+        for lay in (_dev(a), _dev(np.pad(a, ((0, 0), (0, 16))))[:, :K]):
+            got = quant.gemm_i8(lay, _dev(w), _dev(a_scale), _dev(w_scale)).cpu().numpy().astype(np.float64)
+            over = np.abs(value) >= 2.0 ** 128
+            assert np.isinf(got[over]).all() and np.array_equal(np.sign(got[over]), np.sign(value[over]))
+            assert (np.abs(got - value)[~over] <= bound[~over]).all(), (sa, sw)
