@@ -304,8 +304,8 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     if (M > kMost || N > kMost) return set_status(JST_ERR_ARG, "gemm_i8: size > 0x7fff0000");
     if (K > 131071) return set_status(JST_ERR_ARG, "gemm_i8: K > 131071 (the sum could exceed 32 bits)");
     if (epilogue < JST_EPI_NONE || epilogue > JST_EPI_BIAS_RELU) return set_status(JST_ERR_ARG, "gemm_i8: unknown epilogue");
-    if ((epilogue & JST_EPI_BIAS) && !bias) return set_status(JST_ERR_ARG, "gemm_i8: bias epilogue without a bias pointer");
     if (M == 0 || N == 0) return JST_OK;
+    if ((epilogue & JST_EPI_BIAS) && !bias) return set_status(JST_ERR_ARG, "gemm_i8: bias epilogue without a bias pointer");
     if (!C || !b_scale || (K > 0 && !B)) return set_status(JST_ERR_ARG, "gemm_i8: null pointer");
     if ((M > 1 && ldc < N) || (N > 1 && K > 0 && ldb < K)) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
     if ((M > 1 && ldc > INT64_MAX / 8 / M) || (N > 1 && ldb > INT64_MAX / 8 / N))

@@ -1,0 +1,33 @@
+"""What the C entry points of the scan, the dropout and the 8-bit products take and refuse, on the host alone."""
+import ctypes
+
+import pytest
+import torch
+
+from jstorch_b200 import _lib
+
+# addresses far apart that nothing reads: a call that is taken ends at the missing device
+G, H0, LEN, OUT, HN, DOUT, DG, DH0 = (0x10_0000_0000 * (i + 1) for i in range(8))
+TAKEN = 0 if torch.cuda.is_available() else 8  # JST_OK, JST_ERR_NO_DEVICE
+
+
+def _gemm(**change):
+    d = _lib.GemmI8Desc()
+    d.M, d.N, d.K = 4, 5, 16
+    d.A, d.lda, d.B, d.ldb, d.C, d.ldc = G, 16, OUT, 16, DG, 5
+    d.a_scale, d.b_scale, d.bias, d.epilogue = H0, HN, DH0, 1
+    for k, v in change.items():
+        setattr(d, k, v)
+    return _lib.load().jst_gemm_i8(ctypes.byref(d))
+
+
+def _linear(x=G, ldx=16, M=4, K=16, w=OUT, ldw=16, ws=HN, N=5, bias=DH0, epilogue=1, y=DG, ldy=5):
+    return _lib.load().jst_linear_i8(x, ldx, M, K, w, ldw, ws, N, bias, epilogue, y, ldy, None)
+
+
+@pytest.mark.parametrize("empty", [{"M": 0}, {"N": 0}])
+def test_an_empty_product_needs_no_pointer(empty):
+    """An empty tensor has no address: neither operands nor the bias of an epilogue."""
+    none = dict.fromkeys(("A", "B", "C", "a_scale", "b_scale", "bias"))
+    assert _gemm(**empty, **none) == TAKEN
+    assert _linear(**empty, x=None, w=None, ws=None, bias=None, y=None) == TAKEN

@@ -50,3 +50,14 @@ def test_scales_whose_product_leaves_the_type(M):
             over = np.abs(value) >= 2.0 ** 128
             assert np.isinf(got[over]).all() and np.array_equal(np.sign(got[over]), np.sign(value[over]))
             assert (np.abs(got - value)[~over] <= bound[~over]).all(), (sa, sw)
+
+
+@pytest.mark.parametrize("M,N", [(5, 0), (0, 3), (0, 0)])
+def test_empty_products_with_a_bias(M, N):
+    import torch
+    from jstorch_b200 import quant
+    w, s, b = torch.zeros((N, 16), dtype=torch.int8, device="cuda"), torch.ones(N, device="cuda"), torch.zeros(N, device="cuda")
+    for relu in (False, True):
+        assert quant.linear_i8(torch.zeros((M, 16), device="cuda"), w, s, bias=b, relu=relu).shape == (M, N)
+        a = torch.zeros((M, 16), dtype=torch.int8, device="cuda")
+        assert quant.gemm_i8(a, w, torch.ones(M, device="cuda"), s, bias=b, relu=relu).shape == (M, N)
