@@ -310,8 +310,11 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     if ((M > 1 && ldc < N) || (N > 1 && K > 0 && ldb < K)) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
     if ((M > 1 && ldc > INT64_MAX / 8 / M) || (N > 1 && ldb > INT64_MAX / 8 / N))
         return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
-    if (K > 0 && ranges_overlap(C, ((M - 1) * ldc + N) * 4, B, (N - 1) * ldb + K))
+    const int64_t span_c = ((M - 1) * ldc + N) * 4, row = (int64_t)N * 4;
+    if (K > 0 && ranges_overlap(C, span_c, B, (N - 1) * ldb + K))
         return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the weight");
+    if (ranges_overlap(C, span_c, b_scale, row) || ((epilogue & JST_EPI_BIAS) && ranges_overlap(C, span_c, bias, row)))
+        return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the channels' scales or bias");
     return JST_OK;
 }
 
@@ -349,6 +352,8 @@ extern "C" int jst_gemm_i8(const jst_gemm_i8_desc* d) {
         if (d->M > 1 && d->lda > INT64_MAX / 8 / d->M) return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
         if (d->K > 0 && ranges_overlap(d->C, ((d->M - 1) * d->ldc + d->N) * 4, d->A, (d->M - 1) * d->lda + d->K))
             return set_status(JST_ERR_ARG, "gemm_i8: C overlaps A");
+        if (ranges_overlap(d->C, ((d->M - 1) * d->ldc + d->N) * 4, d->a_scale, (int64_t)d->M * 4))
+            return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the tokens' scales");
     }
     rc = require_device();
     if (rc) return rc;

@@ -31,3 +31,13 @@ def test_an_empty_product_needs_no_pointer(empty):
     none = dict.fromkeys(("A", "B", "C", "a_scale", "b_scale", "bias"))
     assert _gemm(**empty, **none) == TAKEN
     assert _linear(**empty, x=None, w=None, ws=None, bias=None, y=None) == TAKEN
+
+
+@pytest.mark.parametrize("vector", ["a_scale", "b_scale", "bias"])
+def test_a_product_does_not_overwrite_its_vectors(vector):
+    """Blocks read scales and bias while others write C."""
+    for at in (DG, DG + 76, DG - 12):  # C is 80 bytes
+        assert _gemm(**{vector: at}) == 1 and b"overlaps" in _lib.load().jst_last_error()
+    if vector != "a_scale":
+        assert _linear(**{"b_scale": {"ws": DG + 76}, "bias": {"bias": DG - 16}}[vector]) == 1
+    assert _gemm(bias=DG, epilogue=0, M=0) == TAKEN
