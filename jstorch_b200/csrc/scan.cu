@@ -682,12 +682,13 @@ int check(const ScanArgs& p, int candidate, bool backward) {
     if (p.ld_gates > most || p.ld_out > most) return set_status(JST_ERR_ARG, "scan: size exceeds 64 bits");
     if (!p.gates) return set_status(JST_ERR_ARG, "scan: null gates");
     const int64_t span_g = ((rows - 1) * p.ld_gates + 2 * H) * 4, span_o = ((rows - 1) * p.ld_out + H) * 4;
-    const int64_t state = (int64_t)p.batch * H * 4;
+    const int64_t state = (int64_t)p.batch * H * 4, span_l = p.lengths ? (int64_t)p.batch * 4 : 0;
     if (!backward) {
         if (!p.out) return set_status(JST_ERR_ARG, "scan: null out");
         if (ranges_overlap(p.out, span_o, p.gates, span_g) || (p.h0 && ranges_overlap(p.out, span_o, p.h0, state)) ||
             (p.h_n && (ranges_overlap(p.h_n, state, p.gates, span_g) || ranges_overlap(p.h_n, state, p.out, span_o))) ||
-            (p.h_n && p.h0 && p.h_n != p.h0 && ranges_overlap(p.h_n, state, p.h0, state)))
+            (p.h_n && p.h0 && p.h_n != p.h0 && ranges_overlap(p.h_n, state, p.h0, state)) ||
+            ranges_overlap(p.out, span_o, p.lengths, span_l) || (p.h_n && ranges_overlap(p.h_n, state, p.lengths, span_l)))
             return set_status(JST_ERR_ARG, "scan: an output overlaps an input");
         return JST_OK;
     }
@@ -696,7 +697,8 @@ int check(const ScanArgs& p, int candidate, bool backward) {
     if (p.ld_dgates > most || (p.dout && p.ld_dout > most)) return set_status(JST_ERR_ARG, "scan backward: size exceeds 64 bits");
     const int64_t span_dg = ((rows - 1) * p.ld_dgates + 2 * H) * 4, span_d = p.dout ? ((rows - 1) * p.ld_dout + H) * 4 : 0;
     const struct { const void* at; int64_t bytes; } in[] = {
-        {p.gates, span_g}, {p.out_in, span_o}, {p.dout, span_d}, {p.h0, state}, {p.dh_n, state}};
+        {p.gates, span_g}, {p.out_in, span_o}, {p.dout, span_d}, {p.h0, state}, {p.dh_n, state},
+        {p.lengths, span_l}};
     for (const auto& i : in) {
         if (!i.at) continue;
         if (ranges_overlap(p.dgates, span_dg, i.at, i.bytes)) return set_status(JST_ERR_ARG, "scan backward: dgates overlaps an input");

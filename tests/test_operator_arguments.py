@@ -41,3 +41,21 @@ def test_a_product_does_not_overwrite_its_vectors(vector):
     if vector != "a_scale":
         assert _linear(**{"b_scale": {"ws": DG + 76}, "bias": {"bias": DG - 16}}[vector]) == 1
     assert _gemm(bias=DG, epilogue=0, M=0) == TAKEN
+
+
+def _forward(gates=G, ld=16, seq=3, batch=2, hidden=8, h0=H0, lengths=LEN, out=OUT, ld_out=8, h_n=HN):
+    return _lib.load().jst_scan_forward(gates, ld, seq, batch, hidden, h0, lengths, 0, 0, out, ld_out, h_n, None)
+
+
+def _backward(gates=G, ld=16, seq=3, batch=2, hidden=8, h0=H0, lengths=LEN, out=OUT, ld_out=8, dout=DOUT, ld_dout=8, dh_n=HN,
+              dgates=DG, ld_dg=16, dh0=DH0):
+    return _lib.load().jst_scan_backward(gates, ld, seq, batch, hidden, h0, lengths, 0, 0, out, ld_out, dout, ld_dout, dh_n,
+                                         dgates, ld_dg, dh0, None)
+
+
+@pytest.mark.parametrize("call,where", [(_forward, (OUT, OUT + 188, OUT - 4, HN, HN + 60)),
+                                        (_backward, (DG, DG + 380, DG - 4, DH0, DH0 + 60))])
+def test_a_scan_does_not_overwrite_its_lengths(call, where):
+    """Every block reads them; blocks of one cluster have to read the same."""
+    for at in where:
+        assert call(lengths=at) == 1 and b"overlaps" in _lib.load().jst_last_error()
