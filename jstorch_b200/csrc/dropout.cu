@@ -133,6 +133,8 @@ extern "C" int jst_dropout(const float* x, int64_t ldx, float* y, int64_t ldy, i
         const bool same = x == y && (ldx == ldy || rows == 1);
         if (!same && ranges_overlap(x, ((rows - 1) * ldx + cols) * 4, y, ((rows - 1) * ldy + cols) * 4))
             return set_status(JST_ERR_ARG, "dropout: x and y overlap");
+        if (step && ranges_overlap(step, 8, y, ((rows - 1) * ldy + cols) * 4))
+            return set_status(JST_ERR_ARG, "dropout: y overlaps step");
     }
     int rc = require_device();
     if (rc) return rc;

@@ -59,3 +59,13 @@ def test_a_scan_does_not_overwrite_its_lengths(call, where):
     """Every block reads them; blocks of one cluster have to read the same."""
     for at in where:
         assert call(lengths=at) == 1 and b"overlaps" in _lib.load().jst_last_error()
+
+
+def _dropout(x=G, ldx=8, y=OUT, ldy=8, rows=4, cols=8, p=0.5, step=None):
+    return _lib.load().jst_dropout(x, ldx, y, ldy, rows, cols, p, 1, 2, step, None)
+
+
+def test_dropout_does_not_overwrite_its_step():
+    """Every thread reads it."""
+    for at in (OUT, OUT + 120, OUT - 4):
+        assert _dropout(step=at) == 1 and b"overlaps" in _lib.load().jst_last_error()
