@@ -131,9 +131,10 @@ extern "C" int jst_dropout(const float* x, int64_t ldx, float* y, int64_t ldy, i
         if (rows > 1 && (ldx > INT64_MAX / 8 / rows || ldy > INT64_MAX / 8 / rows))
             return set_status(JST_ERR_ARG, "dropout: size exceeds 64 bits");
         const bool same = x == y && (ldx == ldy || rows == 1);
-        if (!same && ranges_overlap(x, ((rows - 1) * ldx + cols) * 4, y, ((rows - 1) * ldy + cols) * 4))
+        const ByteRows out{y, rows, cols * 4, ldy * 4};
+        if (!same && rows_overlap({x, rows, cols * 4, ldx * 4}, out))
             return set_status(JST_ERR_ARG, "dropout: x and y overlap");
-        if (step && ranges_overlap(step, 8, y, ((rows - 1) * ldy + cols) * 4))
+        if (step && rows_overlap({step, 1, 8, 8}, out))
             return set_status(JST_ERR_ARG, "dropout: y overlaps step");
     }
     int rc = require_device();

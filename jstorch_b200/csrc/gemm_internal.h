@@ -66,7 +66,26 @@ inline bool ranges_overlap(const void* a, int64_t na, const void* b, int64_t nb)
     return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
-// The same in clusters of `cluster` blocks along x.
+// Rows of `width` bytes, `pitch` bytes apart (a vector is one row).
+struct ByteRows {
+    const void* at;
+    int64_t rows, width, pitch;
+    int64_t span() const { return rows > 0 && width > 0 ? (rows - 1) * pitch + width : 0; }
+};
+
+// Whether two sets of rows have a byte in common: column ranges of one matrix have
+// none, though the one's span lies over the other's.
+inline bool rows_overlap(const ByteRows& a, const ByteRows& b) {
+    if (!ranges_overlap(a.at, a.span(), b.at, b.span())) return false;
+    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;  // not looked into
+    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    if ((a.rows == 1 && b.rows == 1) || pitch <= 0) return true;
+    int64_t off = (int64_t)((intptr_t)b.at - (intptr_t)a.at) % pitch;
+    if (off < 0) off += pitch;
+    return off < a.width || off + b.width > pitch;
+}
+
+// launch_dependent in clusters of `cluster` blocks along x.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_dependent_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem,
                                             cudaStream_t s, Args... args) {

@@ -264,9 +264,8 @@ int check_quantize(const float* x, int64_t ldx, int rows, int cols, const int8_t
     if (rows > 1 && (ldx > INT64_MAX / 8 / rows || ldq > INT64_MAX / 8 / rows))
         return set_status(JST_ERR_ARG, "quantize_rows: size exceeds 64 bits");
     if (cols == 0) return JST_OK;
-    const int64_t span_x = ((rows - 1) * ldx + cols) * 4, span_q = (rows - 1) * ldq + cols, span_s = (int64_t)rows * 4;
-    if (ranges_overlap(q, span_q, x, span_x) || ranges_overlap(scale, span_s, x, span_x) ||
-        ranges_overlap(scale, span_s, q, span_q))
+    const ByteRows in{x, rows, (int64_t)cols * 4, ldx * 4}, out{q, rows, cols, ldq}, scales{scale, 1, (int64_t)rows * 4, 0};
+    if (rows_overlap(out, in) || rows_overlap(scales, in) || rows_overlap(scales, out))
         return set_status(JST_ERR_ARG, "quantize_rows: an output overlaps another array");
     return JST_OK;
 }
@@ -310,10 +309,10 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     if ((M > 1 && ldc < N) || (N > 1 && K > 0 && ldb < K)) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
     if ((M > 1 && ldc > INT64_MAX / 8 / M) || (N > 1 && ldb > INT64_MAX / 8 / N))
         return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
-    const int64_t span_c = ((M - 1) * ldc + N) * 4, row = (int64_t)N * 4;
-    if (K > 0 && ranges_overlap(C, span_c, B, (N - 1) * ldb + K))
+    const ByteRows out{C, M, (int64_t)N * 4, ldc * 4}, scale{b_scale, 1, (int64_t)N * 4, 0}, plus{bias, 1, (int64_t)N * 4, 0};
+    if (rows_overlap(out, {B, N, K, ldb}))
         return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the weight");
-    if (ranges_overlap(C, span_c, b_scale, row) || ((epilogue & JST_EPI_BIAS) && ranges_overlap(C, span_c, bias, row)))
+    if (rows_overlap(out, scale) || ((epilogue & JST_EPI_BIAS) && rows_overlap(out, plus)))
         return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the channels' scales or bias");
     return JST_OK;
 }
@@ -350,9 +349,10 @@ extern "C" int jst_gemm_i8(const jst_gemm_i8_desc* d) {
         if (!d->a_scale || (d->K > 0 && !d->A)) return set_status(JST_ERR_ARG, "gemm_i8: null pointer");
         if (d->M > 1 && d->K > 0 && d->lda < d->K) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
         if (d->M > 1 && d->lda > INT64_MAX / 8 / d->M) return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
-        if (d->K > 0 && ranges_overlap(d->C, ((d->M - 1) * d->ldc + d->N) * 4, d->A, (d->M - 1) * d->lda + d->K))
+        const ByteRows out{d->C, d->M, (int64_t)d->N * 4, d->ldc * 4};
+        if (rows_overlap(out, {d->A, d->M, d->K, d->lda}))
             return set_status(JST_ERR_ARG, "gemm_i8: C overlaps A");
-        if (ranges_overlap(d->C, ((d->M - 1) * d->ldc + d->N) * 4, d->a_scale, (int64_t)d->M * 4))
+        if (rows_overlap(out, {d->a_scale, 1, (int64_t)d->M * 4, 0}))
             return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the tokens' scales");
     }
     rc = require_device();
@@ -373,7 +373,7 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
         if (K > 0 && !x) return set_status(JST_ERR_ARG, "linear_i8: null pointer");
         if (M > 1 && ldx < K) return set_status(JST_ERR_ARG, "linear_i8: pitch too small");
         if (M > 1 && ldx > INT64_MAX / 8 / M) return set_status(JST_ERR_ARG, "linear_i8: size exceeds 64 bits");
-        if (K > 0 && ranges_overlap(y, ((M - 1) * ldy + N) * 4, x, ((M - 1) * ldx + K) * 4))
+        if (rows_overlap({y, M, (int64_t)N * 4, ldy * 4}, {x, M, (int64_t)K * 4, ldx * 4}))
             return set_status(JST_ERR_ARG, "linear_i8: y overlaps x");
     }
     rc = require_device();

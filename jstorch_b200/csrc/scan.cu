@@ -681,32 +681,29 @@ int check(const ScanArgs& p, int candidate, bool backward) {
         return set_status(JST_ERR_ARG, "scan: pitch >= 2^24");
     if (p.ld_gates > most || p.ld_out > most) return set_status(JST_ERR_ARG, "scan: size exceeds 64 bits");
     if (!p.gates) return set_status(JST_ERR_ARG, "scan: null gates");
-    const int64_t span_g = ((rows - 1) * p.ld_gates + 2 * H) * 4, span_o = ((rows - 1) * p.ld_out + H) * 4;
-    const int64_t state = (int64_t)p.batch * H * 4, span_l = p.lengths ? (int64_t)p.batch * 4 : 0;
+    const int64_t state = (int64_t)p.batch * H * 4;
+    auto vector = [](const void* at, int64_t bytes) { return ByteRows{at, at ? 1 : 0, bytes, bytes}; };
+    auto matrix = [&](const void* at, int64_t cols, int64_t ld) { return ByteRows{at, at ? rows : 0, 4 * cols, 4 * ld}; };
+    const ByteRows gates = matrix(p.gates, 2 * H, p.ld_gates), h0 = vector(p.h0, state),
+                   lengths = vector(p.lengths, (int64_t)p.batch * 4);
     if (!backward) {
         if (!p.out) return set_status(JST_ERR_ARG, "scan: null out");
-        if (ranges_overlap(p.out, span_o, p.gates, span_g) || (p.h0 && ranges_overlap(p.out, span_o, p.h0, state)) ||
-            (p.h_n && (ranges_overlap(p.h_n, state, p.gates, span_g) || ranges_overlap(p.h_n, state, p.out, span_o))) ||
-            (p.h_n && p.h0 && p.h_n != p.h0 && ranges_overlap(p.h_n, state, p.h0, state)) ||
-            ranges_overlap(p.out, span_o, p.lengths, span_l) || (p.h_n && ranges_overlap(p.h_n, state, p.lengths, span_l)))
+        const ByteRows out = matrix(p.out, H, p.ld_out), h_n = vector(p.h_n, state);
+        if (rows_overlap(out, gates) || rows_overlap(out, h0) || rows_overlap(out, lengths) || rows_overlap(h_n, gates) ||
+            rows_overlap(h_n, out) || rows_overlap(h_n, lengths) || (p.h_n != p.h0 && rows_overlap(h_n, h0)))
             return set_status(JST_ERR_ARG, "scan: an output overlaps an input");
         return JST_OK;
     }
     if (!p.out_in || !p.dgates) return set_status(JST_ERR_ARG, "scan backward: null out or dgates");
     if (p.ld_dgates < 2 * H || (p.dout && p.ld_dout < H)) return set_status(JST_ERR_ARG, "scan backward: pitch too small");
     if (p.ld_dgates > most || (p.dout && p.ld_dout > most)) return set_status(JST_ERR_ARG, "scan backward: size exceeds 64 bits");
-    const int64_t span_dg = ((rows - 1) * p.ld_dgates + 2 * H) * 4, span_d = p.dout ? ((rows - 1) * p.ld_dout + H) * 4 : 0;
-    const struct { const void* at; int64_t bytes; } in[] = {
-        {p.gates, span_g}, {p.out_in, span_o}, {p.dout, span_d}, {p.h0, state}, {p.dh_n, state},
-        {p.lengths, span_l}};
-    for (const auto& i : in) {
-        if (!i.at) continue;
-        if (ranges_overlap(p.dgates, span_dg, i.at, i.bytes)) return set_status(JST_ERR_ARG, "scan backward: dgates overlaps an input");
-        if (p.dh0 && !(i.at == p.dh0 && i.at == p.dh_n) && ranges_overlap(p.dh0, state, i.at, i.bytes))
+    const ByteRows dgates = matrix(p.dgates, 2 * H, p.ld_dgates), dh0 = vector(p.dh0, state), dh_n = vector(p.dh_n, state);
+    for (const ByteRows& in : {gates, matrix(p.out_in, H, p.ld_out), matrix(p.dout, H, p.ld_dout), h0, dh_n, lengths}) {
+        if (rows_overlap(dgates, in)) return set_status(JST_ERR_ARG, "scan backward: dgates overlaps an input");
+        if (!(in.at == p.dh0 && in.at == p.dh_n) && rows_overlap(dh0, in))
             return set_status(JST_ERR_ARG, "scan backward: dh0 overlaps an input");
     }
-    if (p.dh0 && ranges_overlap(p.dh0, state, p.dgates, span_dg))
-        return set_status(JST_ERR_ARG, "scan backward: dh0 overlaps dgates");
+    if (rows_overlap(dh0, dgates)) return set_status(JST_ERR_ARG, "scan backward: dh0 overlaps dgates");
     return JST_OK;
 }
 

@@ -8,6 +8,7 @@ from jstorch_b200 import _lib
 
 # addresses far apart that nothing reads: a call that is taken ends at the missing device
 G, H0, LEN, OUT, HN, DOUT, DG, DH0 = (0x10_0000_0000 * (i + 1) for i in range(8))
+SHARED = 0x10_0000_0000 * 20
 TAKEN = 0 if torch.cuda.is_available() else 8  # JST_OK, JST_ERR_NO_DEVICE
 
 
@@ -69,3 +70,34 @@ def test_dropout_does_not_overwrite_its_step():
     """Every thread reads it."""
     for at in (OUT, OUT + 120, OUT - 4):
         assert _dropout(step=at) == 1 and b"overlaps" in _lib.load().jst_last_error()
+
+
+def _quantize(x=G, ldx=16, rows=4, cols=16, q=OUT, ldq=16, scale=HN):
+    return _lib.load().jst_quantize_rows_i8(x, ldx, rows, cols, q, ldq, scale, None)
+
+
+@pytest.mark.skipif(TAKEN == 0, reason="calls that are taken run, and these addresses are nobody's")
+def test_column_ranges_of_one_matrix_are_no_overlap():
+    """Operand and output in the same rows of one buffer, side by side."""
+    for call, one, other in (
+            (lambda a, b: _forward(gates=a, ld=24, out=b, ld_out=24), 64, 32),
+            (lambda a, b: _backward(gates=a, ld=32, dgates=b, ld_dg=32), 64, 64),
+            (lambda a, b: _backward(out=a, ld_out=24, dgates=b, ld_dg=24), 32, 64),
+            (lambda a, b: _backward(dout=a, ld_dout=24, dgates=b, ld_dg=24), 32, 64),
+            (lambda a, b: _dropout(x=a, ldx=16, y=b, ldy=16), 32, 32),
+            (lambda a, b: _gemm(A=a, lda=36, C=b, ldc=9), 16, 20),
+            (lambda a, b: _gemm(B=a, ldb=36, C=b, ldc=9), 16, 20),
+            (lambda a, b: _linear(x=a, ldx=21, y=b, ldy=21), 64, 20),
+            (lambda a, b: _quantize(x=a, ldx=20, q=b, ldq=80), 64, 16)):
+        for a, b in ((SHARED, SHARED + one), (SHARED + other, SHARED)):
+            assert call(a, b) == TAKEN
+        for a, b in ((SHARED, SHARED + one - 4), (SHARED + other - 4, SHARED), (SHARED + 4, SHARED)):  # a column in both
+            assert call(a, b) == 1 and b"overlap" in _lib.load().jst_last_error()
+
+
+def test_other_pitches_and_vectors_within_a_matrix_are():
+    """Rows of different pitches cross sooner or later; a vector of several rows' length covers what lies between."""
+    assert _dropout(x=G, ldx=16, y=G + 32, ldy=17) == 1
+    assert _forward(gates=G, ld=32, h_n=G + 64) == TAKEN or TAKEN == 0  # 64 bytes between two rows' gates
+    assert _forward(gates=G, ld=24, h_n=G + 64) == 1
+    assert _gemm(C=G, ldc=9, a_scale=G + 24) == 1
