@@ -22,8 +22,8 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
-#include <mutex>
 
 #include "../../include/jstorch_scan.h"
 #include "gemm_internal.h"
@@ -573,34 +573,51 @@ __global__ void __launch_bounds__(32 * S, BLOCKS) scan_tiled_kernel(const ScanAr
     }
 }
 
+// The largest cluster that tests leave to the device (jst_test_scan_cluster).
+std::atomic<int> test_cluster{kMostBlocks};
+
+// Whether the device places the cluster of `cfg`, which is larger than the 8 that every GPU
+// of the architecture guarantees: it takes a GPC with that many free SMs.  Asked once a
+// device and kernel.
+template <bool BWD, bool TANH, int V, int S, int K, int BLOCKS>
+bool cluster_fits(const cudaLaunchConfig_t& cfg) {
+    static std::atomic<int> known[64] = {};  // 1: yes, 2: no
+    const auto kernel = scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    int answer = known[dev].load(std::memory_order_relaxed);
+    if (answer == 0) {
+        int clusters = 0;
+        const bool fits = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                          cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+        if (!fits) cudaGetLastError();
+        answer = fits ? 1 : 2;
+        known[dev].store(answer, std::memory_order_relaxed);
+    }
+    return answer == 1 && (int)cfg.attrs[0].val.clusterDim.x <= test_cluster.load(std::memory_order_relaxed);
+}
+
 template <bool BWD, bool TANH, int V, int S, int K, int BLOCKS>
 int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
     const int64_t tiles = ((int64_t)p.batch * p.hidden + 32 * V - 1) / (32 * V);
+    const auto kernel = scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>;
+    cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * C));
     cfg.blockDim = dim3(32 * S);
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)C;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (C > 8) {  // more than every GPU of the architecture guarantees
-        static bool attr_set[64] = {};
-        static std::mutex mu;
-        int dev = 0;
-        cudaGetDevice(&dev);
-        std::lock_guard<std::mutex> lk(mu);
-        if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-            if (cudaFuncSetAttribute(scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>,
-                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-                return set_status(JST_ERR_CUDA, "cudaFuncSetAttribute(scan_tiled_kernel) failed");
-            attr_set[dev] = true;
-        }
-    }
+    auto clusters_of = [&](int c) {
+        C = c;
+        cfg.gridDim = dim3((unsigned)(tiles * c));
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)c;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    };
+    clusters_of(C);
+    if (C > 8 && !cluster_fits<BWD, TANH, V, S, K, BLOCKS>(cfg)) clusters_of(8);
     ProfScope prof(s, KID_SCAN);
-    return cudaLaunchKernelEx(&cfg, scan_tiled_kernel<BWD, TANH, V, S, K, BLOCKS>, p, C) == cudaSuccess
+    return cudaLaunchKernelEx(&cfg, kernel, p, C) == cudaSuccess
                ? JST_OK
                : set_status(JST_ERR_CUDA, "scan launch failed");
 }
@@ -723,6 +740,9 @@ int launched(const char* what) {
 
 }  // namespace
 }  // namespace jst
+
+// For tests: clusters of at most `blocks` blocks, as on a device that places no larger ones.
+extern "C" void jst_test_scan_cluster(int blocks) { jst::test_cluster = blocks; }
 
 extern "C" int jst_scan_forward(const float* gates, int64_t ld_gates, int seq, int batch, int hidden, const float* h0,
                                 const int32_t* lengths, int reverse, int candidate, float* out, int64_t ld_out,

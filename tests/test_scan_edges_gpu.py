@@ -88,3 +88,24 @@ def test_gradients_where_tanh_saturates(seq, batch, hidden):
     h0, dh_n = (rng.standard_normal((batch, hidden)).astype(np.float32) for _ in range(2))
     _, _, dgates, _ = _check(gates, h0, rng.standard_normal((seq, batch, hidden)).astype(np.float32), dh_n, tanh=True)
     assert (dgates[..., hidden:].cpu().numpy() != 0)[np.abs(gates[..., hidden:]) < 30].all()
+
+
+def test_a_device_without_room_for_large_clusters():
+    """32 channels and a long axis take clusters of 16 blocks where the device places
+    them, and otherwise of 8: the call works, and within the same bounds."""
+    import ctypes
+
+    from jstorch_b200 import _lib
+    rng = np.random.default_rng(5)
+    gates = rng.standard_normal((1500, 1, 64)).astype(np.float32)
+    h0, dh_n = (rng.standard_normal((1, 32)).astype(np.float32) for _ in range(2))
+    dout = rng.standard_normal((1500, 1, 32)).astype(np.float32)
+    limit = _lib.load().jst_test_scan_cluster
+    limit.argtypes, limit.restype = [ctypes.c_int], None
+    try:
+        for blocks in (16, 8):
+            limit(blocks)
+            for tanh in (False, True):
+                _check(gates, h0, dout, dh_n, tanh=tanh)
+    finally:
+        limit(16)
