@@ -48,6 +48,8 @@ const Tensor& tensor(PyObject* o, const char* name, at::ScalarType type, const c
     if (x.scalar_type() != type)
         type_error(std::string(name) + " must be " + type_name + " (got " + at::toString(x.scalar_type()) + ")");
     if (!x.is_cuda()) value_error(std::string(name) + " must live on a CUDA device");
+    // imag() of a conjugate: the memory holds the values' negatives
+    if (x.is_neg()) value_error(std::string(name) + " is a negated view: give a tensor of its own (resolve_neg())");
     return x;
 }
 const Tensor& f32(PyObject* o, const char* name) { return tensor(o, name, at::kFloat, "float32"); }

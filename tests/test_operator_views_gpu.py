@@ -52,3 +52,23 @@ def test_operands_and_outputs_side_by_side_in_one_buffer(gap):
         assert np.array_equal(buf[:, gap:gap + K].cpu().numpy(), x)
         jstorch_b200.dropout(buf[:, gap:gap + N], 0.5, 3, out=y)
         assert np.array_equal(y.cpu().numpy(), oracle.dropout_f32(x[:, :N], 0.5, 3))
+
+
+def test_a_negated_view_is_refused():
+    """The memory behind the imaginary part of a conjugate holds the negatives of its values."""
+    import torch
+
+    import jstorch_b200
+    from jstorch_b200 import quant, rnn
+    x = torch.randn((6, 1), dtype=torch.complex64, device="cuda").conj().imag
+    assert x.is_neg()
+    w, one = torch.ones((1, 1), dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda")
+    gates = torch.randn((6, 2, 2), dtype=torch.complex64, device="cuda").conj().imag
+    out = torch.zeros((6, 1), device="cuda")
+    for call in (lambda: quant.quantize_rows(x), lambda: quant.linear_i8(x, w, one), lambda: jstorch_b200.dropout(x, 0.5, 1),
+                 lambda: jstorch_b200.dropout(out, 0.5, 1, out=x), lambda: rnn.gated_scan(gates),
+                 lambda: quant.linear_i8(out, w, one, bias=x[0])):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    y = x.resolve_neg()
+    assert bool(((quant.linear_i8(x.resolve_neg(), w, one) - y).abs() <= 1e-6 * y.abs()).all())
