@@ -184,13 +184,20 @@ def launch_count() -> int:
 
 
 def calls():
-    """The extension module _calls (csrc/calls.cpp); raises if it is not built."""
+    """The extension module _calls (csrc/calls.cpp); raises if it is not built, or
+    built for another torch than the one in use (their classes may differ)."""
     global _calls
     if _calls is None:
-        import torch  # noqa: F401  (the libraries that the extension is linked to)
+        import torch  # the libraries that the extension is linked to
 
         load()
-        from . import _calls as module
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise ImportError(f"jstorch_b200._calls cannot be loaded ({e}); run `python -m jstorch_b200.build`") from e
+        if module.torch_version != torch.__version__:
+            raise ImportError(f"jstorch_b200._calls is built for torch {module.torch_version}, in use is {torch.__version__}; "
+                              "run `python -m jstorch_b200.build`")
         _calls = module
     return _calls
 

@@ -123,23 +123,28 @@ CALLS_EXT = PKG / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 def build_calls(force: bool = False, verbose: bool = False) -> Path:
     """_calls: torch tensors to the scan, dropout and quant entry points of
-    libjstorch_gemm.so (found next to it at run time)."""
+    libjstorch_gemm.so (found next to it at run time).  It belongs to one build of
+    torch, whose version it carries, and is built again for another."""
     import torch
 
     BUILD.mkdir(exist_ok=True)
     root = Path(torch.__file__).parent
+    stamp = BUILD / "calls.torch"
+    force = force or not stamp.exists() or stamp.read_text() != torch.__version__
     src, o = CSRC / "calls.cpp", BUILD / "calls.o"
     headers = [INCLUDE / f"jstorch_{n}.h" for n in ("gemm", "scan", "dropout", "quant")]
     if force or not _newer(o, [src] + headers + [Path(__file__)]):
         _run([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", f"-I{CUDA_HOME}/include",
               f"-I{sysconfig.get_paths()['include']}", "-isystem", str(root / "include"), "-isystem",
               str(root / "include/torch/csrc/api/include"),
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-c", str(src), "-o", str(o)], verbose)
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+              f'-DJST_TORCH_VERSION="{torch.__version__}"', "-c", str(src), "-o", str(o)], verbose)
     if force or not _newer(CALLS_EXT, [o, GEMM_LIB]):
         tmp = CALLS_EXT.with_suffix(".tmp")
         _run([CXX, "-shared", "-o", str(tmp), str(o), f"-L{PKG}", "-ljstorch_gemm", f"-L{root / 'lib'}", "-ltorch_python",
               "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"], verbose)
         os.replace(tmp, CALLS_EXT)
+        stamp.write_text(torch.__version__)
     return CALLS_EXT
 
 

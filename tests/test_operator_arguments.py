@@ -101,3 +101,26 @@ def test_other_pitches_and_vectors_within_a_matrix_are():
     assert _forward(gates=G, ld=32, h_n=G + 64) == TAKEN or TAKEN == 0  # 64 bytes between two rows' gates
     assert _forward(gates=G, ld=24, h_n=G + 64) == 1
     assert _gemm(C=G, ldc=9, a_scale=G + 24) == 1
+
+
+def test_another_torch_needs_another_build(monkeypatch):
+    """The extension is bound to one build of torch: not used with another, and built again for it."""
+    from jstorch_b200 import build
+    build.build_calls()
+    assert _lib.calls().torch_version == torch.__version__
+    commands = []
+    monkeypatch.setattr(build, "_run", lambda cmd, verbose: commands.append(cmd))
+    monkeypatch.setattr(build.os, "replace", lambda a, b: None)
+    build.build_calls()
+    assert not commands
+    monkeypatch.setattr(_lib, "_calls", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    with pytest.raises(ImportError, match="jstorch_b200.build"):
+        _lib.calls()
+    stamp = build.BUILD / "calls.torch"
+    held = stamp.read_text()
+    try:
+        build.build_calls()
+        assert len(commands) == 2 and any("0.0.1" in part for part in commands[0])
+    finally:
+        stamp.write_text(held)
