@@ -152,7 +152,6 @@ class GRU(_LayerDropout):
         stream = torch.cuda.current_stream().cuda_stream
         h_n = torch.empty((self.num_layers * dirs, batch, H), dtype=torch.float32, device=x.device)
         call = self.calls
-        self.calls += 1
         inps, outs, saved = [], [], []
         inp = x
         for l in range(self.num_layers):
@@ -172,6 +171,7 @@ class GRU(_LayerDropout):
             saved.append(sv)
             inp = self._drop(out, call, l)
         ctx = _TrainContext(seq, batch, inps, outs, saved, h0, call)
+        self.calls += 1  # a refused call takes no masks
         output = inp.transpose(0, 1) if self.batch_first else inp
         return output, h_n, ctx
 
@@ -329,7 +329,6 @@ class GatedRNN(_LayerDropout):
             raise ValueError("h0 must be a contiguous [num_layers * num_directions, batch, hidden]")
         h_n = torch.empty((self.num_layers * dirs, batch, H), dtype=torch.float32, device=x.device)
         call = self.calls
-        self.calls += 1 if train else 0
         inps, outs, saved, inp = [], [], [], x
         for l in range(self.num_layers):
             out = torch.empty((seq, batch, H * dirs), dtype=torch.float32, device=x.device)
@@ -347,6 +346,7 @@ class GatedRNN(_LayerDropout):
         ctx = _TrainContext(seq, batch, inps, outs, saved, h0, call) if train else None
         if train:
             ctx.lengths = lengths
+            self.calls += 1  # a refused call takes no masks
         return inp.transpose(0, 1) if self.batch_first else inp, h_n, ctx
 
     def __call__(self, x, h0=None, lengths=None):
