@@ -42,18 +42,23 @@ class _TrainContext:
 
 class _LayerDropout:
     """Dropout between stacked layers: layer l of the model's n-th training
-    pass has the mask of (seed, offset n * num_layers + l).  A captured graph
-    repeats the pass that it was captured in, masks included."""
+    pass has the mask of (seed, offset n * num_layers + l + *mask_step).
+
+    A captured graph repeats the pass that it was captured in: its masks too,
+    unless mask_step, an int64 CUDA tensor of one element on the model's device
+    (None: 0), is set before the capture and advanced by num_layers behind the
+    pass's backward(), in the graph.  Every replay then draws the masks that the
+    next pass would."""
 
     def _init_dropout(self, dropout: float, seed: int) -> None:
         if not 0.0 <= dropout <= 1.0:
             raise ValueError(f"dropout must be in [0, 1] (got {dropout})")
-        self.dropout, self.seed, self.calls = dropout, seed, 0
+        self.dropout, self.seed, self.calls, self.mask_step = dropout, seed, 0, None
 
     def _drop(self, x, call: int, layer: int):
         if self.dropout == 0.0 or layer == self.num_layers - 1:
             return x
-        return drop(x, self.dropout, self.seed, call * self.num_layers + layer)
+        return drop(x, self.dropout, self.seed, call * self.num_layers + layer, step=self.mask_step)
 
 
 class GRU(_LayerDropout):
