@@ -109,3 +109,26 @@ def test_a_device_without_room_for_large_clusters():
                 _check(gates, h0, dout, dh_n, tanh=tanh)
     finally:
         limit(16)
+
+
+# every form with lengths: one lane an axis, two channels a lane in rows of several sequences, small blocks,
+# doubled clusters, the backward pass's blocks of four warps, one channel a lane
+@pytest.mark.parametrize("seq,batch,hidden", [(9, 5, 64), (16, 300, 6), (70, 40, 64), (90, 333, 10), (33, 300, 130), (64, 700, 60),
+                                              (1100, 6, 512), (1000, 40, 256), (1100, 40, 256), (2500, 2, 700), (40, 400, 51), (20, 128, 1024)])
+@pytest.mark.parametrize("reverse,tanh", [(False, True), (True, False)])
+def test_lengths_in_every_form(seq, batch, hidden, reverse, tanh):
+    """Sequences of no step, one, some and all, whose ends fall inside a tile, with anything behind them."""
+    rng = np.random.default_rng([seq, batch, hidden])
+    lengths = rng.integers(0, seq + 1, batch).astype(np.int32)
+    lengths[:5] = [seq, 0, 1, seq - 1, seq // 2][:batch]
+    gates = rng.standard_normal((seq, batch, 2 * hidden), dtype=np.float32)
+    gates[..., :hidden] += 2 * rng.standard_normal(hidden, dtype=np.float32)
+    dout = rng.standard_normal((seq, batch, hidden), dtype=np.float32)
+    behind = np.arange(seq)[:, None] >= lengths
+    gates[behind] = np.resize(np.array([np.nan, np.inf, -np.inf, 3e38], np.float32), 2 * hidden)
+    dout[behind] = np.nan
+    h0, dh_n = (rng.standard_normal((batch, hidden), dtype=np.float32) for _ in range(2))
+    out, h_n, dgates, dh0 = _check(gates, h0, dout, dh_n, reverse, tanh, lengths)
+    none = lengths == 0
+    assert np.array_equal(h_n.cpu().numpy()[none], h0[none]) and np.array_equal(dh0.cpu().numpy()[none], dh_n[none])
+    assert not out.cpu().numpy()[behind].any() and not dgates.cpu().numpy()[behind].any()
