@@ -308,7 +308,7 @@ class GatedRNN(_LayerDropout):
     def _project(self, x, l: int, sfx: str, serving: bool):
         """x [..., in] -> gates [..., 2H] of layer l."""
         w, b = f"weight_l{l}{sfx}", self.params[f"bias_l{l}{sfx}"]
-        rows = x.reshape(-1, x.shape[-1])
+        rows = x.reshape(x.shape[:-1].numel(), x.shape[-1])  # without a feature too
         if serving and self.quantized is not None:
             from .quant import linear_i8
             gates = linear_i8(rows, *self.quantized[w], bias=b)
