@@ -326,6 +326,8 @@ class GatedRNN(_LayerDropout):
         x = x.contiguous()
         seq, batch, H, dirs = x.shape[0], x.shape[1], self.hidden_size, len(self._suffixes())
         if train and lengths is not None:  # rows behind a sequence meet dgates of 0 in the weights' gradient
+            if not isinstance(lengths, torch.Tensor):
+                raise TypeError("lengths must be a torch.Tensor")
             if lengths.shape != (batch,) or lengths.device != x.device:
                 raise ValueError(f"lengths must be a contiguous int32 tensor of shape {(batch,)} on {x.device}")
             behind = torch.arange(seq, device=x.device)[:, None] >= lengths

@@ -25,3 +25,12 @@ def test_no_input_features():
     dgates, _ = rnn.gated_scan_backward(gates, first, dfirst)
     assert (model.grads["bias_l0"] - dgates.sum((0, 1))).abs().max() <= 1e-5
     assert torch.equal(model.quantize()(x)[1][0], h_n[0])
+
+
+def test_lengths_of_another_kind():
+    import torch
+    from jstorch_b200 import rnn
+    model, x = rnn.GatedRNN(4, 6), torch.zeros((3, 2, 4), device="cuda")
+    for call in (model, model.forward_train):
+        with pytest.raises(TypeError, match="lengths"):
+            call(x, None, [3, 1])
