@@ -131,10 +131,10 @@ extern "C" int jst_dropout(const float* x, int64_t ldx, float* y, int64_t ldy, i
         if (rows > 1 && (ldx > INT64_MAX / 8 / rows || ldy > INT64_MAX / 8 / rows))
             return set_status(JST_ERR_ARG, "dropout: size exceeds 64 bits");
         const bool same = x == y && (ldx == ldy || rows == 1);
-        const ByteRows out{y, rows, cols * 4, ldy * 4};
-        if (!same && rows_overlap({x, rows, cols * 4, ldx * 4}, out))
+        const ByteRows out = byte_rows(y, rows, cols, ldy, 4);
+        if (!same && rows_overlap(byte_rows(x, rows, cols, ldx, 4), out))
             return set_status(JST_ERR_ARG, "dropout: x and y overlap");
-        if (step && rows_overlap({step, 1, 8, 8}, out))
+        if (step && rows_overlap(byte_rows(step, 1, 1, 1, 8), out))
             return set_status(JST_ERR_ARG, "dropout: y overlaps step");
     }
     int rc = require_device();

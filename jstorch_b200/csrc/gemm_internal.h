@@ -72,6 +72,10 @@ struct ByteRows {
     int64_t rows, width, pitch;
     int64_t span() const { return rows > 0 && width > 0 ? (rows - 1) * pitch + width : 0; }
 };
+// `cols` elements of `size` bytes in each of `rows` rows, `ld` elements apart (one row: any ld).
+inline ByteRows byte_rows(const void* at, int64_t rows, int64_t cols, int64_t ld, int64_t size) {
+    return {at, at ? rows : 0, cols * size, rows > 1 ? ld * size : 0};
+}
 
 // Whether two sets of rows have a byte in common: column ranges of one matrix have
 // none, though the one's span lies over the other's.

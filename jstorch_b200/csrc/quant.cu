@@ -264,7 +264,7 @@ int check_quantize(const float* x, int64_t ldx, int rows, int cols, const int8_t
     if (rows > 1 && (ldx > INT64_MAX / 8 / rows || ldq > INT64_MAX / 8 / rows))
         return set_status(JST_ERR_ARG, "quantize_rows: size exceeds 64 bits");
     if (cols == 0) return JST_OK;
-    const ByteRows in{x, rows, (int64_t)cols * 4, ldx * 4}, out{q, rows, cols, ldq}, scales{scale, 1, (int64_t)rows * 4, 0};
+    const ByteRows in = byte_rows(x, rows, cols, ldx, 4), out = byte_rows(q, rows, cols, ldq, 1), scales = byte_rows(scale, 1, rows, rows, 4);
     if (rows_overlap(out, in) || rows_overlap(scales, in) || rows_overlap(scales, out))
         return set_status(JST_ERR_ARG, "quantize_rows: an output overlaps another array");
     return JST_OK;
@@ -309,10 +309,11 @@ int check_product(int M, int N, int K, int64_t ldb, const void* B, const float* 
     if ((M > 1 && ldc < N) || (N > 1 && K > 0 && ldb < K)) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
     if ((M > 1 && ldc > INT64_MAX / 8 / M) || (N > 1 && ldb > INT64_MAX / 8 / N))
         return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
-    const ByteRows out{C, M, (int64_t)N * 4, ldc * 4}, scale{b_scale, 1, (int64_t)N * 4, 0}, plus{bias, 1, (int64_t)N * 4, 0};
-    if (rows_overlap(out, {B, N, K, ldb}))
+    const ByteRows out = byte_rows(C, M, N, ldc, 4);
+    if (rows_overlap(out, byte_rows(B, N, K, ldb, 1)))
         return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the weight");
-    if (rows_overlap(out, scale) || ((epilogue & JST_EPI_BIAS) && rows_overlap(out, plus)))
+    if (rows_overlap(out, byte_rows(b_scale, 1, N, N, 4)) ||
+        ((epilogue & JST_EPI_BIAS) && rows_overlap(out, byte_rows(bias, 1, N, N, 4))))
         return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the channels' scales or bias");
     return JST_OK;
 }
@@ -349,10 +350,10 @@ extern "C" int jst_gemm_i8(const jst_gemm_i8_desc* d) {
         if (!d->a_scale || (d->K > 0 && !d->A)) return set_status(JST_ERR_ARG, "gemm_i8: null pointer");
         if (d->M > 1 && d->K > 0 && d->lda < d->K) return set_status(JST_ERR_ARG, "gemm_i8: pitch too small");
         if (d->M > 1 && d->lda > INT64_MAX / 8 / d->M) return set_status(JST_ERR_ARG, "gemm_i8: size exceeds 64 bits");
-        const ByteRows out{d->C, d->M, (int64_t)d->N * 4, d->ldc * 4};
-        if (rows_overlap(out, {d->A, d->M, d->K, d->lda}))
+        const ByteRows out = byte_rows(d->C, d->M, d->N, d->ldc, 4);
+        if (rows_overlap(out, byte_rows(d->A, d->M, d->K, d->lda, 1)))
             return set_status(JST_ERR_ARG, "gemm_i8: C overlaps A");
-        if (rows_overlap(out, {d->a_scale, 1, (int64_t)d->M * 4, 0}))
+        if (rows_overlap(out, byte_rows(d->a_scale, 1, d->M, d->M, 4)))
             return set_status(JST_ERR_ARG, "gemm_i8: C overlaps the tokens' scales");
     }
     rc = require_device();
@@ -373,7 +374,7 @@ extern "C" int jst_linear_i8(const float* x, int64_t ldx, int M, int K, const in
         if (K > 0 && !x) return set_status(JST_ERR_ARG, "linear_i8: null pointer");
         if (M > 1 && ldx < K) return set_status(JST_ERR_ARG, "linear_i8: pitch too small");
         if (M > 1 && ldx > INT64_MAX / 8 / M) return set_status(JST_ERR_ARG, "linear_i8: size exceeds 64 bits");
-        if (rows_overlap({y, M, (int64_t)N * 4, ldy * 4}, {x, M, (int64_t)K * 4, ldx * 4}))
+        if (rows_overlap(byte_rows(y, M, N, ldy, 4), byte_rows(x, M, K, ldx, 4)))
             return set_status(JST_ERR_ARG, "linear_i8: y overlaps x");
     }
     rc = require_device();

@@ -698,11 +698,10 @@ int check(const ScanArgs& p, int candidate, bool backward) {
         return set_status(JST_ERR_ARG, "scan: pitch >= 2^24");
     if (p.ld_gates > most || p.ld_out > most) return set_status(JST_ERR_ARG, "scan: size exceeds 64 bits");
     if (!p.gates) return set_status(JST_ERR_ARG, "scan: null gates");
-    const int64_t state = (int64_t)p.batch * H * 4;
-    auto vector = [](const void* at, int64_t bytes) { return ByteRows{at, at ? 1 : 0, bytes, bytes}; };
-    auto matrix = [&](const void* at, int64_t cols, int64_t ld) { return ByteRows{at, at ? rows : 0, 4 * cols, 4 * ld}; };
-    const ByteRows gates = matrix(p.gates, 2 * H, p.ld_gates), h0 = vector(p.h0, state),
-                   lengths = vector(p.lengths, (int64_t)p.batch * 4);
+    const int64_t state = (int64_t)p.batch * H;
+    auto vector = [](const void* at, int64_t n) { return byte_rows(at, 1, n, n, 4); };
+    auto matrix = [&](const void* at, int64_t cols, int64_t ld) { return byte_rows(at, rows, cols, ld, 4); };
+    const ByteRows gates = matrix(p.gates, 2 * H, p.ld_gates), h0 = vector(p.h0, state), lengths = vector(p.lengths, p.batch);
     if (!backward) {
         if (!p.out) return set_status(JST_ERR_ARG, "scan: null out");
         const ByteRows out = matrix(p.out, H, p.ld_out), h_n = vector(p.h_n, state);
