@@ -5,10 +5,7 @@
 //   D[r, s] = sum_k R[r, k] S[s, k]     R: 128 rows a tile, S: BN rows a tile
 //
 // Both operands are K-major as they are stored, so no pass over them is
-// needed.  With many tokens R are the tokens and S the channels (C[r, s]).
-// With few tokens the roles are exchanged (SWAP, C[s, r]): the 128-row side
-// of the instruction then holds channels, of which there are plenty, and the
-// BN side holds the tokens, padded to 16, 32 or 64 instead of 128.
+// needed.  R are the tokens and S the channels (C[r, s]).
 //
 // One persistent CTA per SM walks its tiles:
 //   warp 0      TMA producer: 128-byte k-slabs (swizzle-128B) into a
@@ -51,8 +48,7 @@ template <int BN_, int STAGES_>
 struct Cfg {
     static constexpr int BN = BN_;
     static constexpr int STAGES = STAGES_;
-    static constexpr uint32_t ACC_COLS = BN_ < 32 ? 32 : BN_;  // the epilogue reads 32 columns at a time
-    static constexpr uint32_t TMEM_COLS = 2 * ACC_COLS;
+    static constexpr uint32_t TMEM_COLS = 2 * BN_;  // two accumulators
     static constexpr uint32_t R_BYTES = BM * BK;
     static constexpr uint32_t S_BYTES = BN_ * BK;
     static constexpr uint32_t STAGE_BYTES = R_BYTES + S_BYTES;
@@ -62,7 +58,7 @@ struct Cfg {
     static constexpr uint32_t SMEM_BYTES = BAR_OFF + 256 + 768 /*from 256- to 1024-byte alignment*/;
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
     static_assert(S_BYTES % 1024 == 0, "tiles start on swizzle-pattern boundaries");
-    static_assert(TMEM_COLS >= 32 && TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM allocation");
+    static_assert(BN_ >= 32 && TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM allocation");
     static_assert((2 * STAGES_ + 5) * 8 + 8 <= 256, "barrier area");
 };
 
@@ -255,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int buf = i & 1;
                 if (!ptx::mbar_wait(&acce_bar[buf], ((i >> 1) & 1) ^ 1, err)) break;
                 ptx::tc_fence_after();
-                const uint32_t d = tmem_base + buf * C::ACC_COLS;
+                const uint32_t d = tmem_base + buf * BN;
                 for (int kb = 0; kb < num_kb; ++kb, ++g) {
                     const int s = g % STAGES;
                     if (!ptx::mbar_wait(&full_bar[s], (g / STAGES) & 1, err)) {
@@ -286,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int buf = i & 1;
             int r0, s0;
             tile_at(t, p, BN, &r0, &s0);
-            if (!drain_tile<BN, 2>(p, tm_c, tmem_base + buf * C::ACC_COLS, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
+            if (!drain_tile<BN, 2>(p, tm_c, tmem_base + buf * BN, &accf_bar[buf], (i >> 1) & 1, err, r0, s0, q, half,
                                 blk, tab, stores, [&] { ptx::mbar_arrive(&acce_bar[buf]); }))
                 break;
         }
@@ -899,7 +895,7 @@ static int run_tokens(const I8Args& a, const float* x, int64_t ldx, cudaStream_t
 static int run_aligned(const I8Args& a, cudaStream_t s) {
     if (a.M <= 64) return run_tokens(a, nullptr, 0, s);
     // The tile by what it is expected to take, in ns measured on a B200: a k-slab
-    // (8192^3: 384 us in pairs, 602 and 1055 in tiles of 128 and 64 columns) or,
+    // (8192^3: 365 us in pairs, 602 and 1055 in tiles of 128 and 64 columns) or,
     // where K is short, the epilogue (8192 x 8192 x 512: 93, 66, 93) of a tile,
     // times the waves of tiles, and one of each at the ends.  (256 x 8192 x 8192:
     // 31.5, 25.1, 42.1; 128 x 8192 x 8192: 39.9, 25.1, 23.4; 2048^3: 19.4, 16.4,

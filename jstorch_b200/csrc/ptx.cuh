@@ -107,7 +107,8 @@ __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
 
 // 3-D tiled bulk tensor load global -> this CTA's shared memory, completion
 // counted in bytes on `bar`.  Coordinates are element indices {x, y, z}; x
-// (innermost) times 4 bytes is always a multiple of 16 at every call site.
+// (innermost) times the element's bytes (4, or 1 in 8-bit operands) is a multiple
+// of 16 at every call site.
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
