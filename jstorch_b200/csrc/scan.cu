@@ -162,8 +162,9 @@ __device__ __forceinline__ void gate(const F<V>& a, F<V>& z, F<V>& rest) {
 }
 
 // n = tanh(c) = (1 - t) / (1 + t) of |c| with t = exp(-2 |c|), and below 0.6, where
-// 1 - t would lose digits, c + c^3 P(c^2) with P of degree 4 fitted to the
-// relative error (0.05 of 2^-24).  slope: dn/dc, which is 4 t / (1 + t)^2 (where n
+// 1 - t would lose digits, c + c^3 P(c^2) with P of degree 4: the smallest largest
+// relative error over (0, 0.6] (a linear programme over Chebyshev points; 0.047 of
+// 2^-24, and 0.079 with the coefficients rounded to fp32).  slope: dn/dc, which is 4 t / (1 + t)^2 (where n
 // rounds to 1 that keeps its digits, and 1 - n^2 has none) and below 0.6 1 - n^2.
 template <bool TANH, bool SLOPE, int V>
 __device__ __forceinline__ F<V> candidate(const F<V>& c, F<V>& slope) {
