@@ -3,9 +3,9 @@
 //
 // What a call does beside its launch (checks of a handful of tensors, the
 // outputs' allocation, the stream, a dozen C arguments) is what the smallest calls
-// wait for: 1 x 1 x 1024 steps of the scan take 2.4 us on the device, and the
-// host 5.9 us from here, 13.2 from Python over ctypes; 5 x 2048 x 512 of the
-// 8-bit product take 5.4 and the host 4.4, 10.6 from Python.  The functions take all
+// wait for: 1 x 1 x 1024 steps of the scan take 2.6 us on the device, and the
+// host 5.8 us from here, 13.2 from Python over ctypes; a call of 5 x 2048 x 512 of
+// the 8-bit product takes 5.3 us, 4.4 of them the host's, 10.6 from Python.  The functions take all
 // arguments by position; their documentation and defaults stand in rnn.py,
 // dropout.py and quant.py.
 #include <torch/csrc/Exceptions.h>

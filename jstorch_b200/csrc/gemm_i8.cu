@@ -945,8 +945,8 @@ static int run_aligned(const I8Args& a, cudaStream_t s) {
 
 // Up to 16 tokens of so few values that one launch beats two: such calls wait
 // for the host, which spends 4.4 us on this one and 7.5 on a quantisation, its
-// workspace and the product (5 x 2048 x 512; on the device alone 6.7 and 5.6,
-// and 16 x 1024 x 1024, 10.6 and 6.3).  The weight needs no copy.
+// workspace and the product (5 x 2048 x 512: a call takes 5.5 and 9.3 us, and on the
+// device alone 6.2 and 5.5; 2 x 4096 x 1024, 7.2 and 9.5, 7.8 and 5.9).  The weight needs no copy.
 bool gemm_i8_tc_takes_fp32(const I8Args& a) {
     return a.M <= 16 && (int64_t)a.M * a.K <= 4096 && a.K <= i8::TokCfg<16, 4, true>::SLABS * i8::BK &&
            i8::aligned(a.B, a.ldb, a.N);

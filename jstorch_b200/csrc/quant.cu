@@ -18,7 +18,7 @@ namespace {
 // four a thread, between the peak and the quantisation, so x is read once;
 // NV == 0 (rows of more than 32768 values) reads it twice.  Bound by memory: 5
 // bytes a value.  VEC: x and q rows allow 16- and 4-byte accesses.
-// 8192 x 8192 in 59 us (5.7 TB/s; with conversions and a division near a half 76);
+// 8192 x 8192 in 61 us (5.5 TB/s; with conversions and a division near a half 76);
 // 4096 x 1024 in 6.8, which a warp a row does not change.
 template <int NV, bool VEC>
 __global__ void __launch_bounds__(1024)

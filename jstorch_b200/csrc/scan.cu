@@ -14,11 +14,11 @@
 //
 // Bytes a step and channel: forward 8 read, 4 written; backward 16 read, 8
 // written; nothing but the outputs is kept for the backward pass, which makes
-// the gates again.  Reached on a B200 (tanh): 2048 x 16 x 1024 forward 79 us
-// (5.1 TB/s, 0.78 of the measured copy rate), backward 138 us (5.8 TB/s, 0.89);
-// 65536 x 1 x 1024, identity, 184 us (4.4 TB/s) and 286 us (5.6 TB/s), where
+// the gates again.  Reached on a B200 (tanh): 2048 x 16 x 1024 forward 81 us
+// (5.0 TB/s, 0.76 of the measured copy rate), backward 142 us (5.7 TB/s, 0.86);
+// 65536 x 1 x 1024, identity, 189 us (4.3 TB/s) and 289 us (5.6 TB/s), where
 // one tile's rounds follow each other.  Forward, what is left is issue slots:
-// 38 instructions for 12 bytes.
+// some 38 instructions for 12 bytes.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -626,24 +626,24 @@ int launch_tiled(const ScanArgs& p, int C, cudaStream_t s) {
 // Which kernel, and how the time axis is split.  Times in us, tanh, forward
 // and backward, on a B200 (tile: the 32 * V channels of a warp).
 //   * A few steps, or enough channels to fill the SMs by themselves: one lane
-//     walks the axis (4 x 64 x 1024 [seq x batch x hidden]: 2.7 / 3.5, split
-//     over warps 5.7 / 8.8; 16 x 64 x 1024: 6.2 / 8.0, split 6.1 / 10.1;
-//     128 x 256 x 1024: 71 / 136, split 84 / 150).
+//     walks the axis (4 x 64 x 1024 [seq x batch x hidden]: 2.7 / 3.6, split
+//     over warps 5.7 / 8.8; 16 x 64 x 1024: 5.4 / 6.8, split 6.1 / 10.1;
+//     128 x 256 x 1024: 69 / 139, split 84 / 150).
 //   * Many tiles of a short axis: small blocks, of which many fit an SM
 //     (64 x 64 x 1024: 12.3 / 18.5, 33 x 70 x 1024: 11.3 / 14.4 in blocks of 2 warps x 8
 //     steps; 4 x 4: 13.7 / 18.9, 12.7 / 16.4; 8 x 8: 15.1 / 24.8 for the first).
 //   * Otherwise 64 steps a block and round, 8 a lane (2048 x 16 x 1024 forward
-//     79, with 4 steps a lane 100; backward 4 warps x 8 steps 138, 8 x 8 146,
+//     81, with 4 steps a lane 100; backward 4 warps x 8 steps 142, 8 x 8 149,
 //     4 x 4 200), and where the tiles leave SMs empty, clusters that share a
 //     tile's axis: forward 2 blocks fit an SM, backward 1 (4096 x 1 x 4096:
-//     47 / 83 in clusters of 4 / 2, 94 / 122 without).
+//     45 / 77 in clusters of 4 / 2, 94 / 122 without).
 //   * Long sequences of different lengths: twice the clusters, as the tiles of the
 //     longest outlast the others (2048 x 16 x 1024 with lengths drawn evenly:
 //     65 / 110, 78 / 132 without; at 1000 x 64 x 256 it costs, 40 / 68 for 37 / 67).
 //   * So few channels that even clusters of 8 blocks leave SMs empty: one
-//     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 184 / 286
+//     channel a lane, twice the tiles (65536 x 1 x 1024, identity: 189 / 289
 //     against 240 / 428 with two), and where even those leave half the SMs empty,
-//     clusters of 16 (20000 x 1 x 32, identity: 24.8 / 32.1 for 41.0 / 56.3; with
+//     clusters of 16 (20000 x 1 x 32, identity: 26.0 / 32.9 for 41.0 / 56.3; with
 //     32 tiles they cost, 270 for 190, as fewer such clusters find room).
 template <bool BWD, bool TANH, int V>
 int run_scan(const ScanArgs& p, cudaStream_t s) {
