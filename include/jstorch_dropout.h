@@ -26,7 +26,8 @@ extern "C" {
  *   step     NULL, or a device int64 that is added to offset (modulo 2^64)
  *            when the kernel runs: a captured graph that advances it gets a
  *            new mask at every replay
- *   y        may be x itself (with ldy == ldx); other overlaps are refused
+ *   y        may be x itself (with ldy == ldx), or lie beside x in the same rows;
+ *            what shares a byte with x otherwise, or with step, is refused
  * Asynchronous on `stream`; needs no workspace.
  */
 int jst_dropout(const float* x, int64_t ldx, float* y, int64_t ldy, int64_t rows, int64_t cols, double p,

@@ -14,7 +14,9 @@ values, and backward(ctx, dout, dh_n) runs jst_gru_layer_backward per layer
 and direction, last layer first: parameter gradients accumulate into
 self.grads (as .grad does; zero_grad() clears them) and the gradients of x
 and h0 are returned.  dropout > 0 drops the output of every layer but the last
-in forward_train (include/jstorch_dropout.h); forward() never drops.
+in forward_train (include/jstorch_dropout.h); forward() never drops.  Every
+pass has masks of its own; in a captured graph, which repeats one pass, they
+come from mask_step (a device counter; see _LayerDropout).
 
 gated_scan / gated_scan_backward run the recurrence h_t = z_t h_{t-1} +
 (1 - z_t) n_t on given gate pre-activations; GatedRNN is the layer around it
