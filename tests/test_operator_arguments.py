@@ -98,7 +98,6 @@ def test_column_ranges_of_one_matrix_are_no_overlap():
 def test_other_pitches_and_vectors_within_a_matrix_are():
     """Rows of different pitches cross sooner or later; a vector of several rows' length covers what lies between."""
     assert _dropout(x=G, ldx=16, y=G + 32, ldy=17) == 1
-    assert _forward(gates=G, ld=32, h_n=G + 64) == TAKEN or TAKEN == 0  # 64 bytes between two rows' gates
     assert _forward(gates=G, ld=24, h_n=G + 64) == 1
     assert _gemm(C=G, ldc=9, a_scale=G + 24) == 1
 
